@@ -124,7 +124,7 @@ def work(case):
     if case["kind"] == "plan":
         taken = sum(_blocks(h + n) - _blocks(h) for h, n in zip(held, fresh))
         items = sum((h + n - 1) // BLOCK - h // BLOCK + 1 for h, n in zip(held, fresh) if n)
-        return {"bytes": r * 4 * 5 + taken * 8 + tokens * 12 + items * 8 + 24, "flops": tokens + 4 * r}
+        return {"bytes": r * 4 * 6 + taken * 8 + tokens * 12 + items * 8 + 24, "flops": tokens + 4 * r}
     kv, d = case["kv_heads"], case["head_dim"]
     if case["kind"] == "append":
         full = sum((h + n) // BLOCK - h // BLOCK for h, n in zip(held, fresh))
@@ -212,6 +212,7 @@ def _prepare_plan(case, seed):
                 free_count=_i32([blocks - used]), table=table, length_out=torch.empty_like(_i32(held)),
                 free_count_out=_i32([0]), cu_tokens=torch.empty(r + 1, dtype=torch.int32, device="cuda"),
                 cu_blocks=torch.empty(r + 1, dtype=torch.int32, device="cuda"),
+                cu_items=torch.empty(r + 1, dtype=torch.int32, device="cuda"),
                 slots=torch.empty(room, dtype=torch.int64, device="cuda"),
                 pos=torch.empty(room, dtype=torch.int32, device="cuda"),
                 items=torch.empty((items, 2), dtype=torch.int32, device="cuda"),
@@ -376,6 +377,7 @@ def _plain_plan(s):
     s["free_count_out"].copy_(s["free_count"] - cb[-1:])
     s["cu_tokens"].copy_(cu)
     s["cu_blocks"].copy_(cb)
+    s["cu_items"].copy_(ci)
     s["status"].copy_(torch.stack([code, cu[-1], ci[-1], cb[-1]]))
 
 
@@ -466,7 +468,7 @@ def _own_call(s):
     kind = s["kind"]
     if kind == "plan":
         rc = ta.kv8_plan(s["n_new"], s["length"], s["length_out"], s["free_list"], s["free_count"], s["free_count_out"],
-                         s["table"], s["cu_tokens"], s["cu_blocks"], s["slots"], s["pos"], s["items"], s["status"])
+                         s["table"], s["cu_tokens"], s["cu_blocks"], s["cu_items"], s["slots"], s["pos"], s["items"], s["status"])
     elif kind == "append":
         rc = ta.kv8_append(s["cache"], s["k_new"], s["v_new"], s["cu_tokens"], s["items"])
     elif kind == "attend":
@@ -485,7 +487,8 @@ def run(state):
         _own_call(state)
     else:
         {"plan": _plain_plan, "append": _plain_append, "attend": _plain_attend, "linear": _plain_linear}[kind](state)
-    names = {"plan": ("table", "length_out", "free_count_out", "cu_tokens", "cu_blocks", "slots", "pos", "items", "status"),
+    names = {"plan": ("table", "length_out", "free_count_out", "cu_tokens", "cu_blocks", "cu_items", "slots", "pos",
+                      "items", "status"),
              "append": ("k", "v", "scales", "k_tail", "v_tail"), "attend": ("o",), "linear": ("a", "a_scales", "y")}[kind]
     return {n: state[n] for n in names}
 
