@@ -641,6 +641,185 @@ int tsfm_kv_append_attend(tsfm_kv_cache *cache, const void *k, int64_t k_tok, in
                           int64_t v_tok, int64_t v_batch, const void *q, int64_t q_tok, int64_t q_batch, void *o,
                           int64_t o_tok, int64_t o_batch, int32_t n_new, float scale, uint32_t flags, void *stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Serving in 8 bits: a paged K/V cache with one scale per block of 64 tokens and head, and a matrix
+ * product of e4m3 operands with one scale per block of 128. No counterpart in the reference (it keeps
+ * no cache and computes in f32). tsfm_kv_* above holds 16-bit K/V of one length for every series in
+ * memory of its own; these calls hold half the bytes, any mix of lengths, in the caller's memory.
+ *
+ * One step of a server: tsfm_kv8_plan (block tables and slot maps from the requests' new token counts)
+ * -> q, k, v (tsfm_f8_quantize + tsfm_f8_gemm_nt, or any other product) -> tsfm_kv8_append ->
+ * tsfm_kv8_attend. The requests' tokens are packed: request r's new tokens are rows
+ * cu_tokens[r] .. cu_tokens[r + 1] - 1 of q, k, v and o.
+ *
+ * All of these take device pointers only (flags must hold TSFM_ATTN_DEVICE_PTRS; without it they return
+ * TSFM_E_UNSUPPORTED), allocate nothing, keep nothing between calls, queue kernels on `stream` and
+ * return, so they can be captured into a HIP graph and called from any thread. Pointers belong to the
+ * stream's device (the current one for the NULL stream), whichever device is current. Lengths, tables
+ * and counts are read on the device when the kernels run; out-of-range values there (a table entry that
+ * is no block, a count past max_tokens) never make a kernel touch memory outside the arrays. */
+enum { TSFM_CODE_E4M3 = 0, TSFM_CODE_I8 = 1 }; /* 8-bit element: OCP e4m3 or a signed integer */
+#define TSFM_KV8_BLOCK 64         /* tokens of a cache block */
+#define TSFM_KV8_MAX_REQUESTS 65536
+
+/* The cache, by value in the calls that use it: the caller's arrays. len holds every request's tokens
+ * with those of the step (tsfm_kv8_plan's len_out). The len / 64 whole blocks of a request are held in
+ * 8 bits, in the pool blocks that its table row names; the tokens after them (up to 63) in 16 bits, in the
+ * request's tail: a block gets its scale from all of its 64 tokens at once, so the cache's contents do not
+ * depend on how the tokens were dealt to calls, and no token is rounded twice.
+ * Codes: value = code * scale. E4M3: scale the smallest power of two with absmax / scale <= 448 (at least
+ * 2^-126; 1 for a block of zeros), codes rounded to nearest even: one rounding, at most 2^-4 of a value.
+ * I8: scale = absmax * (1 / 127), code = rint(x * (127 * (1 / absmax))), each operation in f32 and absmax taken as
+ * at least 2^-100 (1 for a block of zeros). A block
+ * whose K (or V) holds a NaN or an infinity gets the scale NaN: every row that reads it becomes NaN.
+ * tsfm_kv8_attend takes any positive scales. */
+typedef struct tsfm_kv8_cache {
+    int32_t dtype;        /* of the tokens, q, o and the tails: TSFM_DTYPE_BF16 or TSFM_DTYPE_F16 */
+    int32_t code;         /* TSFM_CODE_* */
+    int32_t requests;     /* rows of the tails, the table and len; 1 .. TSFM_KV8_MAX_REQUESTS */
+    int32_t kv_heads;
+    int32_t head_dim;     /* 64 or 128 */
+    int32_t blocks;       /* of the pool */
+    int32_t table_width;  /* blocks that a request can have */
+    void *k;              /* (blocks, kv_heads, 64 tokens, head_dim) codes */
+    void *v;              /* (blocks, kv_heads, head_dim, 64) codes: token 32 c + 16 a + 4 g + i (c, a < 2; g, i < 4)
+                             at byte 16 g + 8 c + 4 a + i, the matrix instruction's operand order */
+    float *scales;        /* (blocks, kv_heads, 2): of K and of V */
+    void *k_tail, *v_tail;      /* (requests, kv_heads, 64 tokens, head_dim) of dtype */
+    const int32_t *table;       /* (requests, table_width) pool blocks */
+    const int32_t *len;         /* (requests) */
+} tsfm_kv8_cache;
+
+/* Block tables and slot maps from request lengths. Request r holds len[r] tokens and gets n_new[r] more
+ * (negative: none). It takes the pool blocks it lacks from the end of the free list, requests in order:
+ * block i of all that the step takes is free_list[free_count - 1 - i]. Writes the new table entries and
+ *   cu_tokens, cu_blocks, cu_items: (requests + 1) prefix sums of new tokens, blocks taken, and cache blocks
+ *     that the new tokens touch;
+ *   len_out = len + n_new, free_count_out (either may be the input itself: a captured step advances);
+ *   slots[t] = 64 * block + offset and pos[t] = position in its request (the row of a RoPE table), for each
+ *     packed token t; -1 from the last token to max_tokens;
+ *   items[i] = (request, block index in its table row) for each touched block, in order; (-1, -1) to max_items;
+ *   status: {0, tokens, items, blocks taken}.
+ * All or nothing: where the step cannot be served, status[0] says why (1: more than max_tokens tokens, 2: a
+ * request that passes its table row, or a negative length, 3: not enough free blocks), the counts are 0, and
+ * tables, lengths and the free list are as before: the step's other calls then do nothing.
+ * free_list (blocks) holds the free pool blocks' ids in its first free_count entries. */
+typedef struct tsfm_kv8_plan_args {
+    int32_t requests, blocks, table_width;
+    int32_t max_tokens;   /* entries of slots and pos; 1 .. 2^30 */
+    int32_t max_items;    /* entries of items, at least min(max_tokens, max_tokens / 64 + 2 * requests) */
+    uint32_t flags;       /* TSFM_ATTN_DEVICE_PTRS */
+    const int32_t *n_new, *len;
+    int32_t *len_out;
+    const int32_t *free_list, *free_count;
+    int32_t *free_count_out;
+    int32_t *table;       /* (requests, table_width) */
+    int32_t *cu_tokens, *cu_blocks, *cu_items;
+    int64_t *slots;
+    int32_t *pos;
+    int32_t *items;       /* (max_items, 2) */
+    int32_t *status;      /* (4) */
+    void *stream;
+} tsfm_kv8_plan_args;
+
+int tsfm_kv8_plan(const tsfm_kv8_plan_args *args);
+
+/* Ends requests: for every r with drop[r] != 0 the blocks of its table row (those that are pool blocks)
+ * go back to the end of the free list, requests in order, its entries become -1 and len[r] 0. status[0] = 0,
+ * or 1 and nothing changed where the list would pass `blocks` entries; status[1]: the blocks returned. */
+typedef struct tsfm_kv8_release_args {
+    int32_t requests, blocks, table_width;
+    uint32_t flags;
+    const uint8_t *drop;  /* (requests) */
+    int32_t *len, *table, *free_list, *free_count;
+    int32_t *status;      /* (2) */
+    void *stream;
+} tsfm_kv8_release_args;
+
+int tsfm_kv8_release(const tsfm_kv8_release_args *args);
+
+/* Writes the step's K/V into the cache: element (t, h, c) of k at k[t * k_tok + h * head_dim + c], v alike.
+ * cu_tokens and items are tsfm_kv8_plan's. A touched block that is whole now is quantised (its first tokens
+ * from the tail, if earlier steps brought them), the tokens of one that is not go to the tail. A request
+ * without new tokens, and tail rows behind its last token, are left as they are. Not for the same cache on
+ * two streams at once. */
+typedef struct tsfm_kv8_append_args {
+    tsfm_kv8_cache cache;
+    int32_t max_tokens, max_items;  /* rows of k and v; entries of items */
+    uint32_t flags;
+    const int32_t *cu_tokens, *items;
+    const void *k; int64_t k_tok;   /* strides in elements, multiples of 16 bytes */
+    const void *v; int64_t v_tok;
+    void *stream;
+} tsfm_kv8_append_args;
+
+int tsfm_kv8_append(const tsfm_kv8_append_args *args);
+
+/* Causal attention of the step's queries over the cache: the query of a request's new token i sits at
+ * position p = len - n_new + i and reads keys 0 .. p; query head h reads K/V head h / (heads / kv_heads):
+ *   o[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j
+ * in f32 from the cache's values, rounded once to dtype. A query without keys (a length below its new
+ * tokens) gives 0; rows of o past the last token are left as they are. A token of the tail whose V holds a
+ * NaN or an infinity makes every row that reads it NaN, and no other.
+ * max_new and max_len (0: unknown) are the largest n_new and len to expect; they pick the kernel and the
+ * split of long contexts, and any values give right results.
+ * workspace: tsfm_kv8_attend_workspace bytes (partial results of split contexts; none: may be NULL), written
+ * before it is read. Calls that may run at the same time, and captured graphs that do, need one each. */
+typedef struct tsfm_kv8_attend_args {
+    tsfm_kv8_cache cache;
+    int32_t heads;        /* query heads: a multiple of kv_heads */
+    int32_t max_tokens;   /* rows of q and o */
+    int32_t max_new, max_len;
+    float scale;          /* >= 0 */
+    uint32_t flags;
+    const int32_t *cu_tokens;
+    const void *q; int64_t q_tok;  /* element (t, h, c) at q[t * q_tok + h * head_dim + c] */
+    void *o; int64_t o_tok;
+    void *workspace;
+    int64_t workspace_bytes;
+    void *stream;
+} tsfm_kv8_attend_args;
+
+int tsfm_kv8_attend(const tsfm_kv8_attend_args *args);
+/* Bytes of workspace that this call needs (from its sizes and hints alone; the pointers are not read), or
+ * -1 for arguments that the call refuses (tsfm_attn_last_error). The count of compute units enters: of the
+ * stream's device. */
+int64_t tsfm_kv8_attend_workspace(const tsfm_kv8_attend_args *args);
+
+/* e4m3 codes of a matrix, one f32 scale per 1 x 128 (group_rows 1: activations) or 128 x 128 (group_rows
+ * 128: weights) group: x[r, c] = codes[r, c] * scales[r / group_rows, c / 128], the scale and rounding of a
+ * cache block in E4M3. Groups at the edges are short. A NaN or an infinity becomes the code of NaN; the
+ * scale is that of the group's finite values. cols a multiple of 16. */
+typedef struct tsfm_f8_quantize_args {
+    int32_t dtype;        /* of x: TSFM_DTYPE_* */
+    int32_t rows, cols;
+    int32_t group_rows;   /* 1 or 128 */
+    uint32_t flags;
+    const void *x; int64_t x_ld;      /* row strides in elements: x's and codes' multiples of 16 bytes */
+    uint8_t *codes; int64_t codes_ld;
+    float *scales; int64_t scales_ld;
+    void *stream;
+} tsfm_f8_quantize_args;
+
+int tsfm_f8_quantize(const tsfm_f8_quantize_args *args);
+
+/* c[m, n] = sum over blocks b of 128 of a_scales[m, b] * b_scales[n / 128, b] * (a[m, :] . b[n, :] over the block),
+ * a (m, k) and b (n, k) e4m3 codes row-major, products and sums in f32, rounded once to out_dtype. k a
+ * multiple of 16; m, n any. Scales of any value. */
+typedef struct tsfm_f8_gemm_args {
+    int32_t m, n, k;
+    int32_t out_dtype;    /* TSFM_DTYPE_* */
+    uint32_t flags;
+    const uint8_t *a; int64_t a_ld;            /* row strides in elements; a_ld and b_ld multiples of 16 */
+    const float *a_scales; int64_t a_scales_ld;  /* (m, ceil(k / 128)) */
+    const uint8_t *b; int64_t b_ld;
+    const float *b_scales; int64_t b_scales_ld;  /* (ceil(n / 128), ceil(k / 128)) */
+    void *c; int64_t c_ld;
+    void *stream;
+} tsfm_f8_gemm_args;
+
+int tsfm_f8_gemm_nt(const tsfm_f8_gemm_args *args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,338 @@
+// Products of e4m3 operands with a scale per block of 128, and their quantisation, on gfx950.
+//
+//   c[m, n] = sum over kb of sa[m, kb] sb[n / 128, kb] P_kb[m, n],   P_kb = sum over k in kb of a[m, k] b[n, k]
+// P_kb comes from the matrix instructions, and one multiply-add per output and kb puts it into the f32 sum with its
+// scale. The 8-bit instructions do not keep 32 bits of a sum: their results are 1.4e-5 of the norm off over 128 normal
+// values (16x16x128 and 16x16x32 alike), as if the products were cut off 2^-17 below the largest. That is far below
+// half a step of bf16 or f16, so 16-bit results use them; f32 results take the same codes as f16 values (exact)
+// through the f16 instructions (9e-9 off), at half the rate. The weights are the instruction's A
+// operand and the activations its B operand, so that a lane's results belong to one m: its scale is one register.
+#include "kv8_device.hpp"
+
+namespace tsfm {
+namespace {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int KB = 128;  // values per scale
+
+__device__ __forceinline__ i32x8 pair(u32x4 lo, u32x4 hi) {
+    return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+}
+// 32 x 32 x 64 and 16 x 16 x 128: A and B hold 32 bytes of a row per lane, in the same order of k.
+// EXACT: as four f16 instructions on 8 bytes each.
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+template <bool EXACT>
+struct Operand {
+    u32x4 h[4];  // f16
+    __device__ __forceinline__ void set(i32x8 x) {
+#pragma unroll
+        for (int s = 0; s < 4; s++) h[s] = decode8<kCodeE4m3, false>((uint32_t)x[2 * s], (uint32_t)x[2 * s + 1]);
+    }
+};
+template <>
+struct Operand<false> {
+    i32x8 x;
+    __device__ __forceinline__ void set(i32x8 v) { x = v; }
+};
+__device__ __forceinline__ f32x16 mul(const Operand<false>& a, const Operand<false>& b, f32x16 c) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a.x, b.x, c, 0, 0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mul(const Operand<false>& a, const Operand<false>& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.x, b.x, c, 0, 0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mul(const Operand<true>& a, const Operand<true>& b, f32x16 c) {
+#pragma unroll
+    for (int s = 0; s < 4; s++)
+        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a.h[s]), __builtin_bit_cast(f16x8, b.h[s]), c, 0,
+                                                   0, 0);
+    return c;
+}
+__device__ __forceinline__ f32x4 mul(const Operand<true>& a, const Operand<true>& b, f32x4 c) {
+#pragma unroll
+    for (int s = 0; s < 4; s++)
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a.h[s]), __builtin_bit_cast(f16x8, b.h[s]), c, 0,
+                                                   0, 0);
+    return c;
+}
+
+// ---- quantisation ----
+
+// Eight values at p as f32. DTYPE: TSFM_DTYPE_*.
+template <int DTYPE>
+__device__ __forceinline__ void load8(const void* x, int64_t at, float (&v)[8]) {
+    if constexpr (DTYPE == 0) {
+        const f32x4 a = ld4(static_cast<const float*>(x) + at), b = ld4(static_cast<const float*>(x) + at + 4);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v[i] = a[i];
+            v[4 + i] = b[i];
+        }
+    } else {
+        const u32x4 w = ld16(static_cast<const uint16_t*>(x) + at);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = half_to_f32<DTYPE == 1>((i & 1) ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu);
+    }
+}
+
+// The largest finite magnitude of eight values.
+__device__ __forceinline__ float amax8(const float (&v)[8]) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float a = fabsf(v[i]);
+        m = fmaxf(m, a <= kFltMax ? a : 0.f);
+    }
+    return m;
+}
+// Their codes. What is no finite number becomes a NaN (the sign kept): the conversion of a NaN.
+__device__ __forceinline__ u32x2 codes8(const float (&v)[8], float mul) {
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) y[i] = fabsf(v[i]) <= kFltMax ? v[i] * mul : __builtin_nanf("");
+    return u32x2{encode4<kCodeE4m3>(y[0], y[1], y[2], y[3]), encode4<kCodeE4m3>(y[4], y[5], y[6], y[7])};
+}
+
+// Rows: 16 lanes per group of 128 values (8 each), four groups per wave. Bound by bytes.
+template <int DTYPE>
+__global__ __launch_bounds__(256) void quantize_rows(F8Quantize p) {
+    const int groups = (p.cols + KB - 1) / KB;
+    const int64_t id = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4, total = (int64_t)p.rows * groups;
+    const int l = threadIdx.x & 15;
+    const int64_t row = id / groups;
+    const int grp = (int)(id % groups), col = grp * KB + 8 * l;
+    const bool in = id < total && col < p.cols;  // cols is a multiple of 16: eight values or none
+    float v[8] = {};
+    if (in) load8<DTYPE>(p.x, row * p.x_ld + col, v);
+    float m = amax8(v);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    float scale, mul;
+    block_scale<kCodeE4m3>(m, scale, mul);
+    if (in) *reinterpret_cast<u32x2*>(p.codes + row * p.codes_ld + col) = codes8(v, mul);
+    if (id < total && l == 0) p.scales[row * p.scales_ld + grp] = scale;
+}
+
+// 128 x 128 tiles (weights, once): one workgroup per tile; 16 lanes per row, 16 rows at a time, read twice.
+template <int DTYPE>
+__global__ __launch_bounds__(256) void quantize_tiles(F8Quantize p) {
+    __shared__ float s_max[4];
+    const int groups = (p.cols + KB - 1) / KB;
+    const int grp = blockIdx.x % groups;
+    const int64_t row0 = (int64_t)(blockIdx.x / groups) * KB;
+    const int l = threadIdx.x & 15, col = grp * KB + 8 * l;
+    const int rows = (int)min((int64_t)KB, p.rows - row0);
+    float m = 0.f, v[8];
+    for (int i = threadIdx.x >> 4; i < rows; i += 16)
+        if (col < p.cols) {
+            load8<DTYPE>(p.x, (row0 + i) * p.x_ld + col, v);
+            m = fmaxf(m, amax8(v));
+        }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+    float scale, mul;
+    block_scale<kCodeE4m3>(m, scale, mul);
+    for (int i = threadIdx.x >> 4; i < rows; i += 16)
+        if (col < p.cols) {
+            load8<DTYPE>(p.x, (row0 + i) * p.x_ld + col, v);
+            *reinterpret_cast<u32x2*>(p.codes + (row0 + i) * p.codes_ld + col) = codes8(v, mul);
+        }
+    if (threadIdx.x == 0) p.scales[(int64_t)(blockIdx.x / groups) * p.scales_ld + grp] = scale;
+}
+
+// ---- products ----
+// OUT: TSFM_DTYPE_*. One result at element `at`.
+template <int OUT>
+__device__ __forceinline__ void store1(void* c, int64_t at, float v) {
+    if constexpr (OUT == 0) static_cast<float*>(c)[at] = v;
+    else static_cast<uint16_t*>(c)[at] = (uint16_t)pack2<OUT == 1>(v, 0.f);
+}
+
+// Few rows of a (16 MT): one workgroup per 16 rows of b, its waves sharing the reduction by blocks of 128 and
+// adding up through LDS in order. b is read once, straight into the operands: bound by its bytes, or by latency.
+constexpr int FW = 8;
+template <int OUT, int MT>
+__global__ __launch_bounds__(64 * FW) void gemm_few(F8Gemm p) {
+    __shared__ float part[FW][MT][64][4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int ql = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * 16, kbs = (p.k + KB - 1) / KB;
+    const int64_t brow = (int64_t)min(n0 + ql, p.n - 1) * p.b_ld;
+    f32x4 acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; t++) acc[t] = f32x4{0, 0, 0, 0};
+    auto load = [&](const uint8_t* row, int kb) {  // the lane's 32 bytes of block kb; 0 past k
+        const int k0 = kb * KB + 32 * g;
+        const u32x4 z = {0, 0, 0, 0};
+        return pair(k0 < p.k ? ld16(row + k0) : z, k0 + 16 < p.k ? ld16(row + k0 + 16) : z);
+    };
+    for (int kb = wave; kb < kbs; kb += FW) {
+        Operand<OUT == 0> b, a;
+        b.set(load(p.b + brow, kb));
+        const float sb = p.b_scales[(int64_t)(n0 / KB) * p.b_scales_ld + kb];
+#pragma unroll
+        for (int t = 0; t < MT; t++) {
+            const int64_t m = min(16 * t + ql, p.m - 1);
+            a.set(load(p.a + m * p.a_ld, kb));
+            const float s = sb * p.a_scales[m * p.a_scales_ld + kb];
+            const f32x4 x = mul(b, a, f32x4{0, 0, 0, 0});
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[t][i] = __builtin_fmaf(s, x[i], acc[t][i]);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; t++) st4(part[wave][t][lane], acc[t]);
+    __syncthreads();
+    for (int t = wave; t < MT; t += FW) {
+        f32x4 sum = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < FW; w++) sum += ld4(part[w][t][lane]);
+        const int m = 16 * t + ql;  // the lane's results: rows n0 + 4 g + i of b
+        if (m < p.m)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (n0 + 4 * g + i < p.n) store1<OUT>(p.c, m * p.c_ld + n0 + 4 * g + i, sum[i]);
+    }
+}
+
+// Tiles of TM x TN, WM x WN waves, a step of 128 values at a time. Both operands go from memory into LDS by DMA
+// (buffer loads whose descriptors end after the tile's rows: what is past m, n or k reads as 0), one step ahead,
+// one barrier per step. LDS rows are the step's 128 bytes with their 16-byte pieces XOR-swizzled by row.
+template <int OUT, int TM, int TN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void gemm_tiles(F8Gemm p) {
+    constexpr int NWV = WM * WN, MT = TM / WM / 32, NT = TN / WN / 32;
+    constexpr uint32_t kStage = (TM + TN) * KB;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kStage];
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lr = lane & 31, lh = lane >> 5;
+    const int mt_n = (p.m + TM - 1) / TM, nt_n = (p.n + TN - 1) / TN;
+    const int id = xcd_remap(blockIdx.x, gridDim.x);
+    const int m0 = (id % mt_n) * TM, n0 = (id / mt_n) * TN;
+    (void)nt_n;
+    const int wm = (wave % WM) * (TM / WM), wn = (wave / WM) * (TN / WN);
+    const int kbs = (p.k + KB - 1) / KB;
+    const int mrows = min(TM, p.m - m0), nrows = min(TN, p.n - n0);
+    const u32x4 a_buf = buf_desc(p.a + (int64_t)m0 * p.a_ld, (uint32_t)((mrows - 1) * p.a_ld + p.k));
+    const u32x4 b_buf = buf_desc(p.b + (int64_t)n0 * p.b_ld, (uint32_t)((nrows - 1) * p.b_ld + p.k));
+    // One DMA instruction of a wave fills 1 KB: 8 rows, lane l piece l % 8 of row l / 8.
+    constexpr int AI = TM / 8 / NWV, BI = TN / 8 / NWV;
+    constexpr uint32_t kOutside = 0x80000000u;  // past every descriptor (the host keeps a tile's rows below 2 GiB)
+    const int srow = lane >> 3, spiece = (lane & 7) ^ (srow & 7);
+    auto stage = [&](int kb, int buf) {
+        const uint32_t st = lds0 + buf * kStage;
+        const bool in = kb * KB + 16 * spiece < p.k;
+#pragma unroll
+        for (int i = 0; i < AI; i++) {
+            const int row = (wave * AI + i) * 8;
+            dma16(a_buf, st + row * KB, in ? (uint32_t)(row + srow) * (uint32_t)p.a_ld + 16u * spiece : kOutside,
+                  (uint32_t)kb * KB);
+        }
+#pragma unroll
+        for (int i = 0; i < BI; i++) {
+            const int row = (wave * BI + i) * 8;
+            dma16(b_buf, st + TM * KB + row * KB,
+                  in ? (uint32_t)(row + srow) * (uint32_t)p.b_ld + 16u * spiece : kOutside, (uint32_t)kb * KB);
+        }
+    };
+    typedef __attribute__((address_space(3))) u32x4* lds_ptr;
+    auto operand = [&](uint32_t base, int row, int s) {  // 32 bytes: pieces 4 s + 2 lh, + 1
+        const uint32_t r = base + row * KB, x = row & 7;
+        return pair(*(lds_ptr)(uintptr_t)(r + 16 * ((4 * s + 2 * lh) ^ x)), *(lds_ptr)(uintptr_t)(r + 16 * ((4 * s + 2 * lh + 1) ^ x)));
+    };
+    f32x16 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) acc[i][j] = f32x16{};
+    const float* sa[MT];
+#pragma unroll
+    for (int i = 0; i < MT; i++) sa[i] = p.a_scales + (int64_t)min(m0 + wm + 32 * i + lr, p.m - 1) * p.a_scales_ld;
+    const float* sb = p.b_scales + (int64_t)(min(n0 + wn, p.n - 1) / KB) * p.b_scales_ld;
+
+    stage(0, 0);
+    for (int kb = 0; kb < kbs; kb++) {
+        float s[MT];
+#pragma unroll
+        for (int i = 0; i < MT; i++) s[i] = sa[i][kb] * sb[kb];
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        if (kb + 1 < kbs) stage(kb + 1, (kb + 1) & 1);
+        const uint32_t st = lds0 + (kb & 1) * kStage;
+        Operand<OUT == 0> a[MT][2];
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) a[i][h].set(operand(st, wm + 32 * i + lr, h));
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            Operand<OUT == 0> b[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) b[h].set(operand(st + TM * KB, wn + 32 * j + lr, h));
+#pragma unroll
+            for (int i = 0; i < MT; i++) {
+                f32x16 x = mul(b[0], a[i][0], f32x16{});
+                x = mul(b[1], a[i][1], x);
+#pragma unroll
+                for (int r = 0; r < 16; r++) acc[i][j][r] = __builtin_fmaf(s[i], x[r], acc[i][j][r]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+        const int m = m0 + wm + 32 * i + lr;
+        if (m >= p.m) continue;
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int n = n0 + wn + 32 * j + 8 * (r >> 2) + 4 * lh + (r & 3);
+                if (n < p.n) store1<OUT>(p.c, m * p.c_ld + n, acc[i][j][r]);
+            }
+    }
+}
+
+template <int OUT>
+hipError_t gemm(const F8Gemm& p, int /*cus*/, hipStream_t s) {
+    if (p.m <= 64) {
+        const dim3 grid((unsigned)((p.n + 15) / 16)), block(64 * FW);
+        if (p.m <= 16) hipLaunchKernelGGL((gemm_few<OUT, 1>), grid, block, 0, s, p);
+        else if (p.m <= 32) hipLaunchKernelGGL((gemm_few<OUT, 2>), grid, block, 0, s, p);
+        else hipLaunchKernelGGL((gemm_few<OUT, 4>), grid, block, 0, s, p);
+        return hipGetLastError();
+    }
+    const int64_t grid = (((int64_t)p.m + 127) / 128) * ((p.n + 127) / 128);
+    if (grid > 0x7fffffff) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((gemm_tiles<OUT, 128, 128, 2, 2>), dim3((unsigned)grid), dim3(256), 0, s, p);
+    return hipGetLastError();
+}
+
+template <int DTYPE>
+hipError_t quantize(const F8Quantize& p, hipStream_t s) {
+    const int64_t groups = (p.cols + KB - 1) / KB;
+    if (p.group_rows == 1) {
+        const int64_t grid = (p.rows * groups + 15) / 16;
+        if (grid > 0x7fffffff) return hipErrorInvalidValue;
+        hipLaunchKernelGGL(quantize_rows<DTYPE>, dim3((unsigned)grid), dim3(256), 0, s, p);
+    } else {
+        const int64_t grid = ((int64_t)p.rows + KB - 1) / KB * groups;
+        if (grid > 0x7fffffff) return hipErrorInvalidValue;
+        hipLaunchKernelGGL(quantize_tiles<DTYPE>, dim3((unsigned)grid), dim3(256), 0, s, p);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_f8_quantize(const F8Quantize& p, int dtype, hipStream_t s) {
+    return dtype == 0 ? quantize<0>(p, s) : dtype == 1 ? quantize<1>(p, s) : quantize<2>(p, s);
+}
+
+hipError_t launch_f8_gemm(const F8Gemm& p, int out_dtype, int cus, hipStream_t s) {
+    return out_dtype == 0 ? gemm<0>(p, cus, s) : out_dtype == 1 ? gemm<1>(p, cus, s) : gemm<2>(p, cus, s);
+}
+
+}  // namespace tsfm

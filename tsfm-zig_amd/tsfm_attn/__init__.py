@@ -48,6 +48,10 @@ DTYPE_F32 = 0
 DTYPE_BF16 = 1
 DTYPE_F16 = 2
 
+CODE_E4M3 = 0  # TSFM_CODE_E4M3
+CODE_I8 = 1  # TSFM_CODE_I8
+KV8_BLOCK = 64  # TSFM_KV8_BLOCK: tokens of a block of the 8-bit cache
+
 DEVICE_PTRS = 1
 FORECAST_HOST_IO = 4  # TSFM_FORECAST_HOST_IO: the forecasts' per-call arrays in host memory
 VARIATE_MAX_ROWS = 256  # TSFM_VARIATE_MAX_ROWS: rows per series of the variate and Timestral forecast calls
@@ -84,6 +88,13 @@ EXPORTS = (
     "tsfm_kv_len",
     "tsfm_kv_append",
     "tsfm_kv_attend",
+    "tsfm_kv8_plan",
+    "tsfm_kv8_release",
+    "tsfm_kv8_append",
+    "tsfm_kv8_attend",
+    "tsfm_kv8_attend_workspace",
+    "tsfm_f8_quantize",
+    "tsfm_f8_gemm_nt",
 )
 
 
@@ -522,6 +533,15 @@ def load(path: Optional[os.PathLike] = None) -> ctypes.CDLL:
     lib.tsfm_sgemm_nt.restype = ci
     lib.tsfm_sgemm_nn.argtypes = [ci, ci, ci, vp, ci, vp, ci, vp, ci, vp]
     lib.tsfm_sgemm_nn.restype = ci
+    for fn in ("plan", "release", "append", "attend"):
+        getattr(lib, "tsfm_kv8_" + fn).argtypes = [vp]
+        getattr(lib, "tsfm_kv8_" + fn).restype = ci
+    lib.tsfm_kv8_attend_workspace.argtypes = [vp]
+    lib.tsfm_kv8_attend_workspace.restype = i64
+    lib.tsfm_f8_quantize.argtypes = [vp]
+    lib.tsfm_f8_quantize.restype = ci
+    lib.tsfm_f8_gemm_nt.argtypes = [vp]
+    lib.tsfm_f8_gemm_nt.restype = ci
     if path is None:
         _lib = lib
     return lib
@@ -1157,6 +1177,318 @@ class KvCache:
             self.close()
         except Exception:
             pass
+
+
+# ---- Serving in 8 bits (no counterpart in the reference) ------------------------------------------
+#
+# Thin calls over torch device tensors: sizes and strides come from the tensors, the argument block is packed in one
+# go. Like the other calls they return the ABI's code; tensors of the wrong type or shape raise ValueError.
+
+
+class Kv8CacheArgs(ctypes.Structure):
+    """``tsfm_kv8_cache`` (include/tsfm_attn.h)."""
+
+    _fields_ = [(f, ctypes.c_int32) for f in ("dtype", "code", "requests", "kv_heads", "head_dim", "blocks",
+                                              "table_width")] + \
+               [(f, ctypes.c_void_p) for f in ("k", "v", "scales", "k_tail", "v_tail", "table", "len")]
+
+
+class Kv8PlanArgs(ctypes.Structure):
+    """``tsfm_kv8_plan_args``."""
+
+    _fields_ = [(f, ctypes.c_int32) for f in ("requests", "blocks", "table_width", "max_tokens", "max_items")] + \
+               [("flags", ctypes.c_uint32)] + \
+               [(f, ctypes.c_void_p) for f in ("n_new", "len", "len_out", "free_list", "free_count", "free_count_out",
+                                               "table", "cu_tokens", "cu_blocks", "cu_items", "slots", "pos", "items",
+                                               "status", "stream")]
+
+
+class Kv8ReleaseArgs(ctypes.Structure):
+    """``tsfm_kv8_release_args``."""
+
+    _fields_ = [(f, ctypes.c_int32) for f in ("requests", "blocks", "table_width")] + [("flags", ctypes.c_uint32)] + \
+               [(f, ctypes.c_void_p) for f in ("drop", "len", "table", "free_list", "free_count", "status", "stream")]
+
+
+class Kv8AppendArgs(ctypes.Structure):
+    """``tsfm_kv8_append_args``."""
+
+    _fields_ = [("cache", Kv8CacheArgs), ("max_tokens", ctypes.c_int32), ("max_items", ctypes.c_int32),
+                ("flags", ctypes.c_uint32), ("cu_tokens", ctypes.c_void_p), ("items", ctypes.c_void_p),
+                ("k", ctypes.c_void_p), ("k_tok", ctypes.c_int64), ("v", ctypes.c_void_p), ("v_tok", ctypes.c_int64),
+                ("stream", ctypes.c_void_p)]
+
+
+class Kv8AttendArgs(ctypes.Structure):
+    """``tsfm_kv8_attend_args``."""
+
+    _fields_ = [("cache", Kv8CacheArgs), ("heads", ctypes.c_int32), ("max_tokens", ctypes.c_int32),
+                ("max_new", ctypes.c_int32), ("max_len", ctypes.c_int32), ("scale", ctypes.c_float),
+                ("flags", ctypes.c_uint32), ("cu_tokens", ctypes.c_void_p), ("q", ctypes.c_void_p),
+                ("q_tok", ctypes.c_int64), ("o", ctypes.c_void_p), ("o_tok", ctypes.c_int64),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64), ("stream", ctypes.c_void_p)]
+
+
+class F8QuantizeArgs(ctypes.Structure):
+    """``tsfm_f8_quantize_args``."""
+
+    _fields_ = [(f, ctypes.c_int32) for f in ("dtype", "rows", "cols", "group_rows")] + [("flags", ctypes.c_uint32)] + \
+               [("x", ctypes.c_void_p), ("x_ld", ctypes.c_int64), ("codes", ctypes.c_void_p),
+                ("codes_ld", ctypes.c_int64), ("scales", ctypes.c_void_p), ("scales_ld", ctypes.c_int64),
+                ("stream", ctypes.c_void_p)]
+
+
+class F8GemmArgs(ctypes.Structure):
+    """``tsfm_f8_gemm_args``."""
+
+    _fields_ = [(f, ctypes.c_int32) for f in ("m", "n", "k", "out_dtype")] + [("flags", ctypes.c_uint32)] + \
+               [(f, ctypes.c_void_p if i % 2 == 0 else ctypes.c_int64)
+                for i, f in enumerate(("a", "a_ld", "a_scales", "a_scales_ld", "b", "b_ld", "b_scales", "b_scales_ld",
+                                       "c", "c_ld"))] + [("stream", ctypes.c_void_p)]
+
+
+def _packer(cls: Any) -> struct.Struct:
+    """The C layout of an argument block (a nested block comes first and is a multiple of its alignment long)."""
+    code = {ctypes.c_int32: "i", ctypes.c_uint32: "I", ctypes.c_float: "f", ctypes.c_int64: "q", ctypes.c_void_p: "P"}
+    fields = []
+    for _, t in cls._fields_:
+        fields += [code[u] for _, u in t._fields_] if issubclass(t, ctypes.Structure) else [code[t]]
+    s = struct.Struct("@" + "".join(fields))
+    assert s.size == ctypes.sizeof(cls)
+    return s
+
+
+_KV8_PLAN_PACK = _packer(Kv8PlanArgs)
+_KV8_RELEASE_PACK = _packer(Kv8ReleaseArgs)
+_KV8_APPEND_PACK = _packer(Kv8AppendArgs)
+_KV8_ATTEND_PACK = _packer(Kv8AttendArgs)
+_F8_QUANTIZE_PACK = _packer(F8QuantizeArgs)
+_F8_GEMM_PACK = _packer(F8GemmArgs)
+
+
+def _want(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _rows_of(x: Any, what: str, width: int) -> int:
+    """The row stride of a tensor of rows of `width` elements, (rows, width) or (rows, heads, head_dim)."""
+    if x.dim() == 3:
+        _want(x.shape[1] * x.shape[2] == width and x.stride(2) == 1 and (x.stride(1) == x.shape[2] or x.shape[1] == 1),
+              f"{what}: rows of {width} consecutive elements")
+    else:
+        _want(x.dim() == 2 and x.shape[1] == width and (x.stride(1) == 1 or width == 1),
+              f"{what}: rows of {width} consecutive elements")
+    return x.stride(0)
+
+
+def _kv8_items(requests: int, tokens: int) -> int:
+    """The most cache blocks that `tokens` new tokens of `requests` requests touch (the rows of ``items``)."""
+    return min(tokens, tokens // KV8_BLOCK + 2 * requests)
+
+
+class Kv8Cache:
+    """``tsfm_kv8_cache`` over the caller's tensors (kept alive, not copied): ``k`` (blocks, kv heads, 64, head dim) and
+    ``v`` (blocks, kv heads, head dim, 64; its token order is the header's) of torch.float8_e4m3fn or int8, ``scales``
+    (blocks, kv heads, 2) f32, ``k_tail`` and ``v_tail`` (requests, kv heads, 64, head dim) bf16 or f16, ``table``
+    (requests, blocks of a request) and ``length`` (requests) int32."""
+
+    def __init__(self, k, v, scales, k_tail, v_tail, table, length):
+        blocks, kv_heads, _, head_dim = k.shape
+        requests = length.shape[0]
+        code = {"torch.float8_e4m3fn": CODE_E4M3, "torch.int8": CODE_I8}.get(str(k.dtype))
+        _want(code is not None and v.dtype == k.dtype, "k and v: torch.float8_e4m3fn or torch.int8")
+        _want(k.shape[2] == KV8_BLOCK and tuple(v.shape) == (blocks, kv_heads, head_dim, KV8_BLOCK), "k or v: shape")
+        _want(tuple(scales.shape) == (blocks, kv_heads, 2) and str(scales.dtype) == "torch.float32", "scales")
+        tail = (requests, kv_heads, KV8_BLOCK, head_dim)
+        _want(tuple(k_tail.shape) == tail and tuple(v_tail.shape) == tail and k_tail.dtype == v_tail.dtype, "tails")
+        _want(table.dim() == 2 and table.shape[0] == requests, "table: (requests, blocks of a request)")
+        _want(str(table.dtype) == str(length.dtype) == "torch.int32", "table and length: int32")
+        parts = (k, v, scales, k_tail, v_tail, table, length)
+        _want(all(t.is_cuda and t.is_contiguous() and t.device == k.device for t in parts),
+              "the cache's tensors: contiguous, on one GPU")
+        self.k, self.v, self.scales, self.k_tail, self.v_tail, self.table, self.length = parts
+        self.requests, self.kv_heads, self.head_dim = requests, kv_heads, head_dim
+        self.blocks, self.table_width, self.dtype = blocks, table.shape[1], k_tail.dtype
+        self._fields = (_dtype_code(k_tail), code, requests, kv_heads, head_dim, blocks, self.table_width,
+                        *(t.data_ptr() for t in parts))
+
+
+def kv8_plan(n_new, length, length_out, free_list, free_count, free_count_out, table, cu_tokens, cu_blocks, cu_items,
+             slots, pos, items, status, stream=None) -> int:
+    """``tsfm_kv8_plan``: block tables and slot maps from the requests' new token counts. All int32 but ``slots``
+    (int64); ``length_out`` may be ``length`` and ``free_count_out`` ``free_count``."""
+    r = n_new.shape[0]
+    ints = (n_new, length, length_out, free_list, free_count, free_count_out, table, cu_tokens, cu_blocks, cu_items,
+            pos, items, status)
+    _want(all(str(t.dtype) == "torch.int32" for t in ints) and str(slots.dtype) == "torch.int64", "int32, slots int64")
+    _want(all(t.is_cuda and t.is_contiguous() for t in ints) and slots.is_cuda and slots.is_contiguous(),
+          "contiguous tensors on the GPU")
+    _want(length.shape[0] == length_out.shape[0] == table.shape[0] == r, "one entry per request")
+    _want(cu_tokens.shape[0] == cu_blocks.shape[0] == cu_items.shape[0] == r + 1, "prefix sums: requests + 1 entries")
+    _want(pos.shape[0] == slots.shape[0] and items.shape[1] == 2 and status.numel() >= 4, "slots, pos, items, status")
+    args = _KV8_PLAN_PACK.pack(r, free_list.shape[0], table.shape[1], slots.shape[0], items.shape[0], DEVICE_PTRS,
+                               n_new.data_ptr(), length.data_ptr(), length_out.data_ptr(), free_list.data_ptr(),
+                               free_count.data_ptr(), free_count_out.data_ptr(), table.data_ptr(),
+                               cu_tokens.data_ptr(), cu_blocks.data_ptr(), cu_items.data_ptr(), slots.data_ptr(),
+                               pos.data_ptr(), items.data_ptr(), status.data_ptr(), _stream_of(n_new, stream) or 0)
+    return int(load().tsfm_kv8_plan(args))
+
+
+def kv8_release(drop, length, table, free_list, free_count, status, stream=None) -> int:
+    """``tsfm_kv8_release``: ends the requests whose ``drop`` (uint8 or bool) is not 0."""
+    ints = (length, table, free_list, free_count, status)
+    _want(all(str(t.dtype) == "torch.int32" for t in ints) and drop.element_size() == 1, "int32, drop of bytes")
+    _want(all(t.is_cuda and t.is_contiguous() for t in (*ints, drop)), "contiguous tensors on the GPU")
+    _want(drop.shape[0] == length.shape[0] == table.shape[0] and status.numel() >= 2, "one entry per request")
+    args = _KV8_RELEASE_PACK.pack(length.shape[0], free_list.shape[0], table.shape[1], DEVICE_PTRS, drop.data_ptr(),
+                                  length.data_ptr(), table.data_ptr(), free_list.data_ptr(), free_count.data_ptr(),
+                                  status.data_ptr(), _stream_of(length, stream) or 0)
+    return int(load().tsfm_kv8_release(args))
+
+
+def kv8_append(cache: Kv8Cache, k, v, cu_tokens, items, stream=None) -> int:
+    """``tsfm_kv8_append``: the K/V of the step's packed tokens, (tokens, kv heads * head dim) rows of any stride, into
+    the cache. ``cu_tokens`` and ``items`` are ``kv8_plan``'s."""
+    _want(k.dtype == v.dtype == cache.dtype and k.shape[0] == v.shape[0], "k and v: the cache's dtype, a row per token")
+    _want(k.is_cuda and v.is_cuda and cu_tokens.is_cuda and items.is_cuda and items.is_contiguous()
+          and cu_tokens.is_contiguous(), "tensors on the GPU")
+    _want(str(cu_tokens.dtype) == str(items.dtype) == "torch.int32" and cu_tokens.shape[0] == cache.requests + 1,
+          "cu_tokens and items: int32, as planned")
+    width = cache.kv_heads * cache.head_dim
+    args = _KV8_APPEND_PACK.pack(*cache._fields, k.shape[0], items.shape[0], DEVICE_PTRS, cu_tokens.data_ptr(),
+                                 items.data_ptr(), k.data_ptr(), _rows_of(k, "k", width), v.data_ptr(),
+                                 _rows_of(v, "v", width), _stream_of(k, stream) or 0)
+    return int(load().tsfm_kv8_append(args))
+
+
+def _kv8_attend_sizes(cache: Kv8Cache, heads: int, tokens: int, max_new: int, max_len: int, scale: float) -> tuple:
+    return (*cache._fields, heads, tokens, max_new, max_len, float(scale), DEVICE_PTRS)
+
+
+def kv8_attend_workspace(cache: Kv8Cache, heads: int, tokens: int, max_new: int = 0, max_len: int = 0,
+                         stream=None) -> int:
+    """``tsfm_kv8_attend_workspace``: bytes of workspace that ``kv8_attend`` with these sizes needs."""
+    args = _KV8_ATTEND_PACK.pack(*_kv8_attend_sizes(cache, heads, tokens, max_new, max_len, 0.0), 0, 0, 0, 0, 0, 0, 0,
+                                 _stream_of(cache.k, stream) or 0)
+    n = int(load().tsfm_kv8_attend_workspace(args))
+    if n < 0:
+        raise TsfmError(E_UNSUPPORTED, last_error())
+    return n
+
+
+def kv8_attend(cache: Kv8Cache, q, o, cu_tokens, *, scale: float, max_new: int = 0, max_len: int = 0, workspace=None,
+               stream=None) -> int:
+    """``tsfm_kv8_attend``: causal attention of the step's packed queries, (tokens, heads, head dim) or (tokens,
+    heads * head dim), over the cache, into ``o`` of the same shape."""
+    width = q.shape[1] * q.shape[2] if q.dim() == 3 else q.shape[1]
+    _want(q.dtype == o.dtype == cache.dtype and o.shape == q.shape, "q and o: the cache's dtype, one shape")
+    _want(q.is_cuda and o.is_cuda and cu_tokens.is_cuda and cu_tokens.is_contiguous(), "tensors on the GPU")
+    _want(str(cu_tokens.dtype) == "torch.int32" and cu_tokens.shape[0] == cache.requests + 1, "cu_tokens: as planned")
+    _want(width % cache.head_dim == 0, "q: whole heads")
+    room = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    args = _KV8_ATTEND_PACK.pack(*_kv8_attend_sizes(cache, width // cache.head_dim, q.shape[0], max_new, max_len, scale),
+                                 cu_tokens.data_ptr(), q.data_ptr(), _rows_of(q, "q", width), o.data_ptr(),
+                                 _rows_of(o, "o", width), 0 if workspace is None else workspace.data_ptr(), room,
+                                 _stream_of(q, stream) or 0)
+    return int(load().tsfm_kv8_attend(args))
+
+
+class Kv8Pool:
+    """A paged 8-bit cache with its block pool, for a server's loop: ``step`` plans the new tokens of every request,
+    ``append`` and ``attend`` run on them, ``release`` ends requests. Nothing waits for the GPU; ``status`` (device)
+    tells whether the last step was served. The calls go to ``stream`` or torch's current one: one stream (or ordered
+    ones) for a pool."""
+
+    def __init__(self, requests: int, blocks: int, kv_heads: int, head_dim: int = 64, *, max_len: int, max_tokens: int,
+                 dtype=None, code: int = CODE_E4M3, device="cuda"):
+        import torch
+
+        dtype = torch.bfloat16 if dtype is None else dtype
+        width = -(-max_len // KV8_BLOCK)
+
+        def empty(*shape, t=torch.int32):
+            return torch.empty(shape, dtype=t, device=device)
+
+        codes = torch.float8_e4m3fn if code == CODE_E4M3 else torch.int8
+        self.cache = Kv8Cache(empty(blocks, kv_heads, KV8_BLOCK, head_dim, t=codes),
+                              empty(blocks, kv_heads, head_dim, KV8_BLOCK, t=codes),
+                              empty(blocks, kv_heads, 2, t=torch.float32),
+                              empty(requests, kv_heads, KV8_BLOCK, head_dim, t=dtype),
+                              empty(requests, kv_heads, KV8_BLOCK, head_dim, t=dtype),
+                              torch.full((requests, width), -1, dtype=torch.int32, device=device),
+                              torch.zeros(requests, dtype=torch.int32, device=device))
+        self.length, self.table = self.cache.length, self.cache.table
+        self.free_list = torch.arange(blocks - 1, -1, -1, dtype=torch.int32, device=device)
+        self.free_count = torch.full((1,), blocks, dtype=torch.int32, device=device)
+        self.cu_tokens, self.cu_blocks, self.cu_items = (
+            torch.zeros(requests + 1, dtype=torch.int32, device=device) for _ in range(3))
+        self.slots, self.pos = empty(max_tokens, t=torch.int64), empty(max_tokens)
+        self.items = torch.full((_kv8_items(requests, max_tokens), 2), -1, dtype=torch.int32, device=device)
+        self.status = torch.zeros(4, dtype=torch.int32, device=device)
+        self._workspace = None
+
+    @staticmethod
+    def _check(rc: int) -> None:
+        if rc != OK:
+            raise TsfmError(rc, last_error())
+
+    def step(self, n_new, stream=None) -> None:
+        """Plans ``n_new`` (requests) new tokens: lengths, tables and maps advance."""
+        self._check(kv8_plan(n_new, self.length, self.length, self.free_list, self.free_count, self.free_count,
+                             self.table, self.cu_tokens, self.cu_blocks, self.cu_items, self.slots, self.pos, self.items,
+                             self.status, stream))
+
+    def append(self, k, v, stream=None) -> None:
+        self._check(kv8_append(self.cache, k, v, self.cu_tokens, self.items, stream))
+
+    def attend(self, q, o, scale: float, max_new: int = 0, max_len: int = 0, workspace=None, stream=None) -> None:
+        """``workspace``: the caller's (a captured step needs one of its own); without one the pool keeps a tensor as
+        large as its largest call needed."""
+        if workspace is None:
+            import torch
+
+            heads = q.numel() // max(1, q.shape[0]) // self.cache.head_dim
+            n = kv8_attend_workspace(self.cache, heads, q.shape[0], max_new, max_len, stream)
+            if n > 0 and (self._workspace is None or self._workspace.numel() < n):
+                self._workspace = torch.empty(n, dtype=torch.uint8, device=q.device)
+            workspace = self._workspace
+        self._check(kv8_attend(self.cache, q, o, self.cu_tokens, scale=scale, max_new=max_new, max_len=max_len,
+                               workspace=workspace, stream=stream))
+
+    def release(self, drop, stream=None) -> None:
+        self._check(kv8_release(drop, self.length, self.table, self.free_list, self.free_count, self.status, stream))
+
+
+def f8_quantize(x, codes, scales, group_rows: int = 1, stream=None) -> int:
+    """``tsfm_f8_quantize``: ``x`` (rows, cols) f32, bf16 or f16 to e4m3 ``codes`` and f32 ``scales`` (ceil(rows /
+    group_rows), ceil(cols / 128)): group_rows 1 for activations, 128 for weights."""
+    rows, cols = x.shape
+    groups, scale_rows = -(-cols // 128), -(-rows // group_rows)
+    _want(x.is_cuda and codes.is_cuda and scales.is_cuda, "tensors on the GPU")
+    _want(codes.shape == x.shape and str(codes.dtype) == "torch.float8_e4m3fn", "codes: torch.float8_e4m3fn as x")
+    _want(tuple(scales.shape) == (scale_rows, groups) and str(scales.dtype) == "torch.float32", "scales: f32 per group")
+    args = _F8_QUANTIZE_PACK.pack(_dtype_code(x), rows, cols, group_rows, DEVICE_PTRS, x.data_ptr(),
+                                  _rows_of(x, "x", cols), codes.data_ptr(), _rows_of(codes, "codes", cols),
+                                  scales.data_ptr(), _rows_of(scales, "scales", groups), _stream_of(x, stream) or 0)
+    return int(load().tsfm_f8_quantize(args))
+
+
+def f8_gemm_nt(a, a_scales, b, b_scales, c, stream=None) -> int:
+    """``tsfm_f8_gemm_nt``: c (m, n) = a (m, k) b (n, k)^T of e4m3 codes with scales (m, ceil(k / 128)) and (ceil(n /
+    128), ceil(k / 128)); c f32, bf16 or f16."""
+    (m, k), n = a.shape, b.shape[0]
+    kb, nb = -(-k // 128), -(-n // 128)
+    _want(all(t.is_cuda for t in (a, a_scales, b, b_scales, c)), "tensors on the GPU")
+    _want(str(a.dtype) == str(b.dtype) == "torch.float8_e4m3fn" and b.shape[1] == k, "a and b: e4m3 codes of one k")
+    _want(tuple(a_scales.shape) == (m, kb) and tuple(b_scales.shape) == (nb, kb)
+          and str(a_scales.dtype) == str(b_scales.dtype) == "torch.float32", "scales: f32 per group")
+    _want(tuple(c.shape) == (m, n), "c: (m, n)")
+    args = _F8_GEMM_PACK.pack(m, n, k, _dtype_code(c), DEVICE_PTRS, a.data_ptr(), _rows_of(a, "a", k),
+                              a_scales.data_ptr(), _rows_of(a_scales, "a_scales", kb), b.data_ptr(),
+                              _rows_of(b, "b", k), b_scales.data_ptr(), _rows_of(b_scales, "b_scales", kb),
+                              c.data_ptr(), _rows_of(c, "c", n), _stream_of(a, stream) or 0)
+    return int(load().tsfm_f8_gemm_nt(args))
 
 
 # ---- Timestral forecast -------------------------------------------------------------------------
