@@ -60,6 +60,7 @@ struct Kv8Attend {
     int32_t chunks;    // workgroups along the keys, per row tile
     int32_t rows;      // rows of a tile
     int32_t kernel;    // kAttend*
+    int32_t once;      // the keys are read past the caches
     float* part;       // partial results: O (rows of o, heads, chunks, D), then (max, sum) pairs
 };
 constexpr int kAttendFew = 0, kAttendMany = 1;

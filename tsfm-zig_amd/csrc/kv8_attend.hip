@@ -8,6 +8,8 @@
 // follows p s_v, the weights that are rounded to 16 bits for the matrix instruction are at most 1 and lose nothing
 // that counts beside the largest product of weight and value scale, whatever the blocks' scales are.
 // Codes become bf16 / f16 in registers, exactly. The tail's values go in as they are (scales 1).
+#include <algorithm>
+
 #include "kv8_device.hpp"
 
 namespace tsfm {
@@ -35,15 +37,59 @@ __device__ __forceinline__ int chunk_blocks(const Kv8Attend& p, int nblk) {
     return max(p.chunk, (nblk + p.chunks - 1) / p.chunks);
 }
 
+// Eight dims of a row's result: to o where its keys were one chunk, else with the row's max and sum to the workspace.
+template <bool BF16, int D>
+__device__ __forceinline__ void store_row(const Kv8Attend& p, const Span& s, int h, int64_t row, int d0, int nchunk, int ck,
+                                          float M, float L, f32x4 a0, f32x4 a1) {
+    const int tok = (int)(row / p.group), hq = h * p.group + (int)(row % p.group);
+    const int64_t at = s.t0 + (int64_t)tok;
+    if (nchunk == 1) {
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        a0 *= inv;
+        a1 *= inv;
+        *reinterpret_cast<u32x4*>(p.o + at * p.o_tok + hq * D + d0) = u32x4{
+            pack2<BF16>(a0[0], a0[1]), pack2<BF16>(a0[2], a0[3]), pack2<BF16>(a1[0], a1[1]), pack2<BF16>(a1[2], a1[3])};
+        return;
+    }
+    const int64_t slot = (at * p.heads + hq) * p.chunks + ck;
+    float* dst = p.part + slot * D + d0;
+    st4(dst, a0);
+    st4(dst + 4, a1);
+    if (d0 == 0)
+        *reinterpret_cast<float2*>(p.part + (int64_t)p.max_tokens * p.heads * p.chunks * D + 2 * slot) = float2{M, L};
+}
+
 // ---- few rows: each wave streams whole blocks from HBM ----
 // One workgroup = (request, K/V head, 16 QT rows, chunk of the keys); its four waves take blocks w, w + 4, ...
 // S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32: a lane's 16-byte loads of K (one key, 16 dims) and V (one
-// dim, 16 tokens in the operand's order) are the operands, so nothing passes through LDS until the waves' results
-// are merged. Bound by HBM.
+// dim, 16 tokens in the operand's order) are the operands, so no block passes through LDS; only the tail's V does,
+// to be transposed. A block's K is loaded again as soon as its scores are formed, its V after its products: what is
+// in flight while a wave computes is the next block.
 constexpr int NW = 4;
 
-template <int CODE, bool BF16, int D, int QT>
-__global__ __launch_bounds__(64 * NW) void attend_few(Kv8Attend p) {
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4* lds_i16x4_ptr;
+// Transposing read: each 16-lane group reads 16 dims of four rows (lane s: row s / 4, dims 4 (s % 4) .. + 3 at its
+// address) and lane s gets dim s of the four.
+__device__ __forceinline__ u32x2 lds_read_tr(uint32_t addr) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_ptr)(uintptr_t)addr));
+}
+
+// 16 bytes of a block; ONCE: past the caches, for a cache larger than they are.
+template <bool ONCE>
+__device__ __forceinline__ u32x4 ld_block(const uint8_t* p) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+    else return ld16(p);
+}
+
+// Waves per SIMD that the few-row kernel is built for: registers of 128, 168 or 256 a wave. Measured either way: 64 dims
+// at three waves 68 us where four take 63 (64 requests of up to 8192 tokens, 32 heads over 8, int8), 128 dims at three
+// (two spills) 144 where two take 134 (two requests of 262144).
+constexpr int few_waves(int d, int qt) { return d == 64 ? (qt == 1 ? 4 : 3) : 2; }
+
+template <int CODE, bool BF16, int D, int QT, bool ONCE>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(few_waves(D, QT), few_waves(D, QT)))) void attend_few(
+    Kv8Attend p) {
     constexpr int R = 16 * QT;      // rows
     constexpr int KU = D / 64;      // 16-byte loads of a key's row per lane
     constexpr int DB = D / 16;      // 16-dim blocks of O
@@ -51,21 +97,31 @@ __global__ __launch_bounds__(64 * NW) void attend_few(Kv8Attend p) {
         float m[NW][R], l[NW][R];
         float o[NW][R][D + 4];
     };
-    __shared__ Merge mg;
+    // The tail's K and V, rows of 2 D bytes whose 16-byte pieces are XOR-swizzled by row (operand reads of 16 rows and
+    // transposing reads of four lie on different banks). The merge uses the same space.
+    constexpr uint32_t kTail = kKvBlock * D * 2;
+    __shared__ __attribute__((aligned(1024))) char lds[sizeof(Merge) > 2 * kTail ? sizeof(Merge) : 2 * kTail];
+    Merge& mg = *reinterpret_cast<Merge*>(lds);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ql = lane & 15, g = lane >> 4;
     const Kv8& c = p.c;
+    // Heads are dealt first, chunks last. Workgroups go to the 8 XCDs in turn: with chunks dealt first, a power of two of
+    // them puts the late chunks, which only long contexts have, on the same XCDs (128 requests of up to 4096 tokens,
+    // chunks of 16 blocks: 146 us, this way 120).
     int id = blockIdx.x;
-    const int ck = id % p.chunks;
-    id /= p.chunks;
+    const int h = id % c.heads;
+    id /= c.heads;
     const int tile0 = id % p.tiles;
     id /= p.tiles;
-    const int h = id % c.heads, r = id / c.heads;
+    const int r = id % c.requests, ck = id / c.requests;
     const Span s = request_span(p.cu_tokens, c.len, r, p.max_tokens, c.width);
     const int G = p.group;
     const int64_t rows = (int64_t)s.n * G;
     const int nfull = s.total / kKvBlock;  // blocks held in 8 bits
+    const int32_t* __restrict__ table = c.table + (int64_t)r * c.width;
+    const int32_t early = table[min(ck * p.chunk + wave, c.width - 1)];  // the wave's first block, most likely
 
     for (int64_t row0 = (int64_t)tile0 * R; row0 < rows; row0 += (int64_t)p.tiles * R) {
         const int last = (int)((min(rows, row0 + R) - 1) / G);  // the tile's last token
@@ -74,6 +130,66 @@ __global__ __launch_bounds__(64 * NW) void attend_few(Kv8Attend p) {
         if (ck >= nchunk) continue;
         const int b0 = ck * cb, b1 = min(nblk, b0 + cb);
         const int first_end = keys_to(s, (int)(row0 / G));  // keys every row of the tile reads
+        const int bq = min(b1, nfull);  // end of the chunk's whole blocks
+
+        u32x4 kc[4][KU], vc[DB];
+        float2 sc;
+        int64_t at;       // the loaded block, in (block, head) units
+        int blk_next = 0;  // table entry of the block after it
+        auto find = [&](int blk) {  // its place; a table entry that is no block: scales of NaN
+            const bool ok = blk >= 0 && blk < c.blocks;
+            at = (int64_t)(ok ? blk : 0) * c.heads + h;
+            sc = reinterpret_cast<const float2*>(c.scales)[at];
+            if (!ok) sc.x = __builtin_nanf("");
+        };
+        // A load instruction covers 1 KB of consecutive bytes: 16 rows of 64, or 8 rows of 128, for which lane bit 3 tells
+        // the half of the row; take_k() then exchanges that bit with the pair of loads, so that as with 64 dims a lane
+        // holds one row's pieces. (Sixteen half rows an instruction: every line asked for twice, 0.88 of the rate.)
+        auto load_k = [&]() {
+            const uint8_t* kb = c.k + at * kKvBlock * D + (KU == 1 ? ql * D : (ql & 7) * D + 8 * (ql & 8)) + 16 * g;
+#pragma unroll
+            for (int kg = 0; kg < 4; kg++)
+#pragma unroll
+                for (int u = 0; u < KU; u++) kc[kg][u] = ld_block<ONCE>(kb + (16 * kg + 8 * u) * D);
+        };
+        auto take_k = [&](int kg) {
+            if constexpr (KU == 2)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    // rotations by 8 within 16 lanes: to lanes 8..15 the second load of lanes 0..7, and the other way round
+                    const int a = (int)kc[kg][0][e], b = (int)kc[kg][1][e];
+                    kc[kg][0][e] = (uint32_t)__builtin_amdgcn_update_dpp(a, b, 0x128, 0xf, 0xc, false);
+                    kc[kg][1][e] = (uint32_t)__builtin_amdgcn_update_dpp(b, a, 0x128, 0xf, 0x3, false);
+                }
+        };
+        auto load_v = [&]() {
+            const uint8_t* vb = c.v + at * kKvBlock * D + ql * kKvBlock + 16 * g;
+#pragma unroll
+            for (int db = 0; db < DB; db++) vc[db] = ld_block<ONCE>(vb + 16 * db * kKvBlock);
+        };
+        int j = b0 + wave;
+        // The tail follows the whole blocks in the deal. Its wave has it copied to LDS now, by DMA, without registers.
+        constexpr int LR = D / 8, RL = 64 / LR;  // lanes per row, rows per 1 KB
+        const bool has_tail = nfull >= b0 && nfull < b1 && (nfull - b0) % NW == wave;
+        if (has_tail) {
+            const uint32_t bytes = (uint32_t)(s.total - nfull * kKvBlock) * D * 2;  // rows past the last token read 0
+            const int64_t at16 = ((int64_t)r * c.heads + h) * kKvBlock * D;
+            const u32x4 kt = buf_desc(c.k_tail + at16, bytes), vt = buf_desc(c.v_tail + at16, bytes);
+            const int row = lane / LR;
+            const uint32_t off[2] = {(uint32_t)row * D * 2 + 16u * ((lane % LR) ^ (row & 7)),
+                                     (uint32_t)row * D * 2 + 16u * ((lane % LR) ^ ((row + RL) & 7))};
+#pragma unroll
+            for (int i = 0; i < kKvBlock / RL; i++) {
+                dma16(kt, lds0 + 1024 * i, off[i & 1], 1024 * i);
+                dma16(vt, lds0 + kTail + 1024 * i, off[i & 1], 1024 * i);
+            }
+        }
+        if (j < bq) {
+            find(cb == p.chunk ? early : table[j]);
+            load_k();
+            load_v();
+            if (j + NW < bq) blk_next = table[j + NW];
+        }
 
         u32x4 qf[QT][2 * KU];
         int kv_end[QT];  // keys of this lane's row
@@ -97,24 +213,8 @@ __global__ __launch_bounds__(64 * NW) void attend_few(Kv8Attend p) {
             for (int db = 0; db < DB; db++) oacc[db][qt] = f32x4{0, 0, 0, 0};
         }
 
-        u32x4 kc[4][KU], vc[DB];
-        float2 sc;
-        auto load = [&](int j) {  // block j of the request (a whole one)
-            const int blk = c.table[(int64_t)r * c.width + j];
-            const bool ok = blk >= 0 && blk < c.blocks;
-            const int64_t at = (int64_t)(ok ? blk : 0) * c.heads + h;
-            const uint8_t* kb = c.k + at * kKvBlock * D;
-            const uint8_t* vb = c.v + at * kKvBlock * D;
-            sc = reinterpret_cast<const float2*>(c.scales)[at];
-            if (!ok) sc.x = __builtin_nanf("");
-#pragma unroll
-            for (int kg = 0; kg < 4; kg++)
-#pragma unroll
-                for (int u = 0; u < KU; u++) kc[kg][u] = ld16(kb + (16 * kg + ql) * D + 64 * u + 16 * g);
-#pragma unroll
-            for (int db = 0; db < DB; db++) vc[db] = ld16(vb + (16 * db + ql) * kKvBlock + 16 * g);
-        };
-        // One block's scores -> weights: t = s kx + lv, masked past the rows' keys; pf: the packed weights.
+        // One block's scores -> weights: t = s kx + lv, masked past the rows' keys; pf: the packed weights. bad: bits
+        // 4 kg + i of the lane's keys whose V is no number.
         auto softmax = [&](f32x4 (&sa)[4][QT], float kx, float lv, int k0, bool plain, uint32_t bad, u32x4 (&pf)[2][QT]) {
             const float inv = __builtin_amdgcn_exp2f(-lv);
 #pragma unroll
@@ -125,8 +225,11 @@ __global__ __launch_bounds__(64 * NW) void attend_few(Kv8Attend p) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         float t = __builtin_fmaf(sa[kg][qt][i], kx, lv);
-                        const int key = k0 + 16 * kg + 4 * g + i;
-                        if (!plain) t = key < kv_end[qt] ? ((bad >> (4 * kg + i)) & 1 ? __builtin_nanf("") : t) : kNegInf;
+                        if (!plain) {
+                            const int key = 16 * kg + 4 * g + i;
+                            if (bad & (1u << (4 * kg + i))) t = __builtin_nanf("");
+                            t = k0 + key < kv_end[qt] ? t : kNegInf;
+                        }
                         sa[kg][qt][i] = t;
                         mloc = fmaxf(mloc, t);
                     }
@@ -155,15 +258,13 @@ __global__ __launch_bounds__(64 * NW) void attend_few(Kv8Attend p) {
             }
         };
 
-        const int bq = min(b1, nfull);  // whole blocks of the chunk
-        int j = b0 + wave;
-        if (j < bq) load(j);
         for (; j < bq; j += NW) {
             f32x4 sa[4][QT];
 #pragma unroll
             for (int kg = 0; kg < 4; kg++) {
 #pragma unroll
                 for (int qt = 0; qt < QT; qt++) sa[kg][qt] = f32x4{0, 0, 0, 0};
+                take_k(kg);
 #pragma unroll
                 for (int u = 0; u < KU; u++) {
                     const u32x4 lo = decode8<CODE, BF16>(kc[kg][u][0], kc[kg][u][1]);
@@ -175,86 +276,109 @@ __global__ __launch_bounds__(64 * NW) void attend_few(Kv8Attend p) {
                     }
                 }
             }
-            u32x4 pf[2][QT], vd[DB];
-            softmax(sa, sc.x * p.c2, __builtin_amdgcn_logf(sc.y), j * kKvBlock, (j + 1) * kKvBlock <= first_end, 0u, pf);
-#pragma unroll
-            for (int db = 0; db < DB; db++) vd[db] = vc[db];
-            if (j + NW < bq) load(j + NW);
+            const float kx = sc.x * p.c2, lv = __builtin_amdgcn_logf(sc.y);
+            const bool more = j + NW < bq;
+            if (more) {
+                find(blk_next);
+                load_k();
+                if (j + 2 * NW < bq) blk_next = table[j + 2 * NW];
+            }
+            u32x4 pf[2][QT];
+            softmax(sa, kx, lv, j * kKvBlock, (j + 1) * kKvBlock <= first_end, 0, pf);
 #pragma unroll
             for (int db = 0; db < DB; db++) {
-                const u32x4 lo = decode8<CODE, BF16>(vd[db][0], vd[db][1]);
-                const u32x4 hi = decode8<CODE, BF16>(vd[db][2], vd[db][3]);
+                const u32x4 lo = decode8<CODE, BF16>(vc[db][0], vc[db][1]);
+                const u32x4 hi = decode8<CODE, BF16>(vc[db][2], vc[db][3]);
 #pragma unroll
                 for (int qt = 0; qt < QT; qt++) {
                     oacc[db][qt] = mfma16<BF16>(lo, pf[0][qt], oacc[db][qt]);
                     oacc[db][qt] = mfma16<BF16>(hi, pf[1][qt], oacc[db][qt]);
                 }
             }
+            if (more) load_v();
         }
-        if (j == nfull && j < b1) {  // the tail: this wave's next block
-            const int live = s.total - nfull * kKvBlock;  // its tokens
-            const uint16_t* kt = c.k_tail + ((int64_t)r * c.heads + h) * kKvBlock * D;
-            const uint16_t* vt = c.v_tail + ((int64_t)r * c.heads + h) * kKvBlock * D;
+        if (has_tail) {
+            // The lane's place, opaque: addresses formed from it are not kept in registers across the loop above.
+            int lane_t = lane;
+            asm volatile("" : "+v"(lane_t));
+            const int ql = lane_t & 15, g = lane_t >> 4;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies; LDS that this wave alone reads: no barrier
+            typedef __attribute__((address_space(3))) u32x4* lds_u32x4_ptr;
+            // V's values that are no numbers become 0, and their tokens' weights NaN in the rows that see them: 0 * NaN
+            // must not reach the rows that do not.
+            uint64_t bad = 0;
+#pragma unroll 2
+            for (int i = 0; i < kKvBlock / RL; i++) {
+                const uint32_t at = lds0 + kTail + 1024 * i + 16 * lane_t;
+                u32x4 x = *(lds_u32x4_ptr)(uintptr_t)at;
+                bool any = false;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    constexpr uint32_t ex = BF16 ? 0x7f80u : 0x7c00u;
+                    const bool lo = (x[e] & ex) == ex, hi = ((x[e] >> 16) & ex) == ex;
+                    any |= lo || hi;
+                    if (lo) x[e] &= 0xffff0000u;
+                    if (hi) x[e] &= 0xffffu;
+                }
+                const uint64_t m = __ballot(any);
+                if (m) {
+                    *(lds_u32x4_ptr)(uintptr_t)at = x;
+                    for (int w = 0; w < RL; w++)
+                        if ((m >> (w * LR)) & ((1ull << LR) - 1)) bad |= 1ull << (RL * i + w);
+                }
+            }
             f32x4 sa[4][QT];
 #pragma unroll
             for (int kg = 0; kg < 4; kg++) {
-                const int t = 16 * kg + ql;
+                const uint32_t krow = lds0 + (16 * kg + ql) * D * 2;
 #pragma unroll
                 for (int qt = 0; qt < QT; qt++) sa[kg][qt] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int u = 0; u < 2 * KU; u++) {
-                    const u32x4 a = t < live ? ld16(kt + t * D + 64 * (u >> 1) + 16 * g + 8 * (u & 1)) : u32x4{0, 0, 0, 0};
+                    const int piece = (8 * (u >> 1) + 2 * g + (u & 1)) ^ (ql & 7);
+                    const u32x4 a = *(lds_u32x4_ptr)(uintptr_t)(krow + 16 * piece);
 #pragma unroll
                     for (int qt = 0; qt < QT; qt++) sa[kg][qt] = mfma16<BF16>(a, qf[qt][u], sa[kg][qt]);
                 }
             }
-            // V: the lane's 8 tokens of a chunk for one dim; values that are no numbers become 0 here, and their
-            // tokens' weights NaN in the rows that see them: 0 * NaN must not reach the rows that do not.
-            u32x4 va[2][DB];
-            uint32_t bad = 0;
+            uint32_t mine = 0;
 #pragma unroll
-            for (int ch = 0; ch < 2; ch++)
-#pragma unroll
-                for (int db = 0; db < DB; db++)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const int t = 32 * ch + (e < 4 ? 4 * g + e : 12 + 4 * g + e);
-                        uint32_t x = t < live ? vt[t * D + 16 * db + ql] : 0;
-                        constexpr uint32_t ex = BF16 ? 0x7f80u : 0x7c00u;
-                        if ((x & ex) == ex) {
-                            bad |= 1u << (8 * ch + e);
-                            x = 0;
-                        }
-                        va[ch][db][e >> 1] = (e & 1) ? va[ch][db][e >> 1] | (x << 16) : x;
-                    }
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) bad |= __shfl_xor((int)bad, o);  // over the 16 lanes of a group: its dims
+            for (int kg = 0; kg < 4; kg++) mine |= ((uint32_t)(bad >> (16 * kg + 4 * g)) & 15u) << (4 * kg);
             u32x4 pf[2][QT];
-            softmax(sa, p.c2, 0.f, nfull * kKvBlock, false, bad, pf);
+            softmax(sa, p.c2, 0.f, nfull * kKvBlock, false, mine, pf);
+            const int vr = 4 * g + (ql >> 2);  // the lane's row of a transposing read (+ 16, 32, 48: the same swizzle)
+            const uint32_t vrow = lds0 + kTail + vr * D * 2 + 8 * (ql & 1);
 #pragma unroll
             for (int db = 0; db < DB; db++)
 #pragma unroll
-                for (int qt = 0; qt < QT; qt++) {
-                    oacc[db][qt] = mfma16<BF16>(va[0][db], pf[0][qt], oacc[db][qt]);
-                    oacc[db][qt] = mfma16<BF16>(va[1][db], pf[1][qt], oacc[db][qt]);
+                for (int ch = 0; ch < 2; ch++) {
+                    const uint32_t a = vrow + 32 * ch * D * 2 + 16 * ((2 * db + ((ql >> 1) & 1)) ^ (vr & 7));
+                    const u32x2 lo = lds_read_tr(a), hi = lds_read_tr(a + 16 * D * 2);
+                    const u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+                    for (int qt = 0; qt < QT; qt++) oacc[db][qt] = mfma16<BF16>(v, pf[ch][qt], oacc[db][qt]);
                 }
         }
 
         // ---- merge the waves' results ----
+        __syncthreads();  // the tail's rows, in the same LDS, have been read
+        int tid_m = tid;  // opaque, as above
+        asm volatile("" : "+v"(tid_m));
+        const int ql_m = tid_m & 15, g_m = (tid_m & 63) >> 4;
 #pragma unroll
         for (int qt = 0; qt < QT; qt++) {
             const float l = sum4(l_run[qt]);
-            const int rr = 16 * qt + ql;
-            if (g == 0) {
+            const int rr = 16 * qt + ql_m;
+            if (g_m == 0) {
                 mg.m[wave][rr] = m_run[qt];
                 mg.l[wave][rr] = l;
             }
 #pragma unroll
-            for (int db = 0; db < DB; db++) st4(&mg.o[wave][rr][16 * db + 4 * g], oacc[db][qt]);
+            for (int db = 0; db < DB; db++) st4(&mg.o[wave][rr][16 * db + 4 * g_m], oacc[db][qt]);
         }
         __syncthreads();
         constexpr int PR = D / 8;  // threads per row
-        for (int i = tid; i < R * PR; i += 64 * NW) {
+        for (int i = tid_m; i < R * PR; i += 64 * NW) {
             const int rr = i / PR, d0 = 8 * (i % PR);
             const int64_t row = row0 + rr;
             if (row >= rows) continue;
@@ -270,37 +394,20 @@ __global__ __launch_bounds__(64 * NW) void attend_few(Kv8Attend p) {
                 a0 += f * ld4(&mg.o[w][rr][d0]);
                 a1 += f * ld4(&mg.o[w][rr][d0 + 4]);
             }
-            const int tok = (int)(row / G), hq = h * G + (int)(row % G);
-            const int64_t at = s.t0 + (int64_t)tok;
-            if (nchunk == 1) {
-                const float inv = L == 0.f ? 0.f : 1.f / L;
-                a0 *= inv;
-                a1 *= inv;
-                *reinterpret_cast<u32x4*>(p.o + at * p.o_tok + hq * D + d0) =
-                    u32x4{pack2<BF16>(a0[0], a0[1]), pack2<BF16>(a0[2], a0[3]), pack2<BF16>(a1[0], a1[1]),
-                          pack2<BF16>(a1[2], a1[3])};
-            } else {
-                const int64_t slot = (at * p.heads + hq) * p.chunks + ck;
-                float* dst = p.part + slot * D + d0;
-                st4(dst, a0);
-                st4(dst + 4, a1);
-                if (d0 == 0)
-                    *reinterpret_cast<float2*>(p.part + (int64_t)p.max_tokens * p.heads * p.chunks * D + 2 * slot) =
-                        float2{M, L};
-            }
+            store_row<BF16, D>(p, s, h, row, d0, nchunk, ck, M, L, a0, a1);
         }
         __syncthreads();  // the next tile's results go to the same LDS
     }
 }
 
 // ---- joining the chunks ----
-// One wave per row of o: the partial results of its chunks, in order.
+// One workgroup per row of o: its four waves take a quarter of the row's chunks each, eight loads in flight, and add up
+// in order.
 template <bool BF16, int D>
 __global__ __launch_bounds__(256) void attend_join(Kv8Attend p) {
-    const int lane = threadIdx.x & 63;
-    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (id >= (int64_t)p.max_tokens * p.heads) return;
-    const int t = (int)(id / p.heads), hq = (int)(id % p.heads);
+    __shared__ float s_l[4], s_o[4][D];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int t = (int)(blockIdx.x / p.heads), hq = (int)(blockIdx.x % p.heads);
     const Kv8& c = p.c;
     // The token's request: t itself where every request has one token, else the last r with cu[r] <= t.
     int r = min(t, c.requests - 1);
@@ -325,7 +432,8 @@ __global__ __launch_bounds__(256) void attend_join(Kv8Attend p) {
     const int n = max(1, (nblk + cb - 1) / cb);
     if (n == 1) return;
     const int64_t slot = ((int64_t)t * p.heads + hq) * p.chunks;
-    const float2* ml = reinterpret_cast<const float2*>(p.part + (int64_t)p.max_tokens * p.heads * p.chunks * D) + slot;
+    const float2* __restrict__ ml = reinterpret_cast<const float2*>(p.part + (int64_t)p.max_tokens * p.heads * p.chunks * D) + slot;
+    const float* __restrict__ part = p.part + slot * D;
     float M = kNegInf;
     for (int k = lane; k < n; k += 64) M = fmaxf(M, ml[k].x);
 #pragma unroll
@@ -333,28 +441,42 @@ __global__ __launch_bounds__(256) void attend_join(Kv8Attend p) {
     float L = 0.f;
     constexpr int E = D / 64;
     float acc[E] = {};
-    for (int k = 0; k < n; k++) {
+    const int k0 = n * wave / 4, k1 = n * (wave + 1) / 4;
+#pragma unroll 8
+    for (int k = k0; k < k1; k++) {
         const float2 x = ml[k];
         const float f = x.x == kNegInf ? 1.f : __builtin_amdgcn_exp2f(x.x - M);
         L += f * x.y;
 #pragma unroll
-        for (int e = 0; e < E; e++) acc[e] += f * p.part[(slot + k) * D + E * lane + e];
+        for (int e = 0; e < E; e++) acc[e] += f * part[(int64_t)k * D + E * lane + e];
     }
+#pragma unroll
+    for (int e = 0; e < E; e++) s_o[wave][E * lane + e] = acc[e];
+    if (lane == 0) s_l[wave] = L;
+    __syncthreads();
+    if (wave) return;
+    L = ((s_l[0] + s_l[1]) + s_l[2]) + s_l[3];
     const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+    for (int e = 0; e < E; e++)
+        acc[e] = (((s_o[0][E * lane + e] + s_o[1][E * lane + e]) + s_o[2][E * lane + e]) + s_o[3][E * lane + e]) * inv;
     uint16_t* dst = p.o + (int64_t)t * p.o_tok + hq * D + E * lane;
-    if constexpr (E == 1) *dst = (uint16_t)pack2<BF16>(acc[0] * inv, 0.f);
-    else *reinterpret_cast<uint32_t*>(dst) = pack2<BF16>(acc[0] * inv, acc[1] * inv);
+    if constexpr (E == 1) *dst = (uint16_t)pack2<BF16>(acc[0], 0.f);
+    else *reinterpret_cast<uint32_t*>(dst) = pack2<BF16>(acc[0], acc[1]);
 }
 
 template <int CODE, bool BF16, int D>
 hipError_t attend(const Kv8Attend& p, hipStream_t s) {
     const int64_t grid = (int64_t)p.c.requests * p.c.heads * p.tiles * p.chunks;
     if (grid <= 0 || grid > 0x7fffffff) return hipErrorInvalidValue;
-    if (p.rows == 16) hipLaunchKernelGGL((attend_few<CODE, BF16, D, 1>), dim3((unsigned)grid), dim3(64 * NW), 0, s, p);
-    else hipLaunchKernelGGL((attend_few<CODE, BF16, D, 2>), dim3((unsigned)grid), dim3(64 * NW), 0, s, p);
+    const dim3 g((unsigned)grid), b(64 * NW);
+    if (p.rows == 16 && p.once) hipLaunchKernelGGL((attend_few<CODE, BF16, D, 1, true>), g, b, 0, s, p);
+    else if (p.rows == 16) hipLaunchKernelGGL((attend_few<CODE, BF16, D, 1, false>), g, b, 0, s, p);
+    else if (p.once) hipLaunchKernelGGL((attend_few<CODE, BF16, D, 2, true>), g, b, 0, s, p);
+    else hipLaunchKernelGGL((attend_few<CODE, BF16, D, 2, false>), g, b, 0, s, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.chunks == 1) return e;
-    const int64_t rows = ((int64_t)p.max_tokens * p.heads + 3) / 4;
+    const int64_t rows = (int64_t)p.max_tokens * p.heads;
     hipLaunchKernelGGL((attend_join<BF16, D>), dim3((unsigned)rows), dim3(256), 0, s, p);
     return hipGetLastError();
 }
@@ -373,17 +495,19 @@ int64_t kv8_attend_plan(Kv8Attend& p, int head_dim, int max_new, int max_len, in
     const int64_t rows = fresh * p.group;
     p.rows = rows <= 16 ? 16 : 32;
     p.kernel = kAttendFew;
+    p.once = (int64_t)p.c.requests * len * p.c.heads * head_dim >= (int64_t)256 << 20;
     const int64_t tiles = (rows + p.rows - 1) / p.rows;
     p.tiles = (int32_t)(tiles < 1024 ? tiles : 1024);
     const int64_t blocks = (len + kKvBlock - 1) / kKvBlock;
     const int64_t base = (int64_t)p.c.requests * p.c.heads * p.tiles;
-    int64_t chunks = 1;
-    const int64_t want = 4 * cus;
-    if (base < want) chunks = (want + base - 1) / base;
-    int64_t chunk = (blocks + chunks - 1) / chunks;
-    if (chunk < 8) chunk = 8;
+    // Split the keys while the workgroups fit the CUs at once: a second round of shorter ones costs more than it fills
+    // (two requests of 262144 tokens, 8 heads of 128: 384 workgroups 134 us, 768 147, 1536 163; 32 requests of up to
+    // 2048 tokens, 16 heads of 64: unsplit 18.3 us, in two with the join 20.2). Chunks are 8 to 128 blocks: shorter ones
+    // are all start and merge, and a longer one would keep a single workgroup busy after the others.
+    const int64_t chunks_wanted = std::max<int64_t>(1, (int64_t)cus * few_waves(head_dim, p.rows / 16) / base);
+    const int64_t chunk = std::min<int64_t>(128, std::max<int64_t>(8, (blocks + chunks_wanted - 1) / chunks_wanted));
+    const int64_t chunks = (blocks + chunk - 1) / chunk;
     p.chunk = (int32_t)chunk;
-    chunks = (blocks + chunk - 1) / chunk;
     p.chunks = (int32_t)chunks;
     if (base * chunks > INT32_MAX || (int64_t)p.max_tokens * p.heads > INT32_MAX) return -1;
     return chunks == 1 ? 0 : (int64_t)p.max_tokens * p.heads * chunks * (head_dim + 2) * 4;
