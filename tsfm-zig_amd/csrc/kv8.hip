@@ -279,7 +279,7 @@ __global__ __launch_bounds__(PT) void release(Kv8Release p) {
 }
 
 // ---- append ----
-// One wave per (touched block, head), for K and V. A lane holds tokens 16 s + 4 g + i (g = lane / 16; s, i < 4) of
+// One wave per (touched block, head, K or V). A lane holds tokens 16 s + 4 g + i (g = lane / 16; s, i < 4) of
 // E = D / 16 dims: a row's 16 lanes read its 2 D bytes together, a lane's four consecutive tokens of one dim pack
 // into the word that V's byte order wants, and the four words of a dim are 16 contiguous bytes of the block: V is
 // transposed in registers, without LDS.
@@ -290,35 +290,24 @@ __global__ __launch_bounds__(256) void kv8_append(Kv8Append p) {
     typedef uint32_t piece __attribute__((ext_vector_type(W)));
     const int lane = threadIdx.x & 63, g = lane >> 4, cl = lane & 15;
     const Kv8& c = p.c;
-    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (id >= (int64_t)p.max_items * c.heads) return;
-    const int h = (int)(id % c.heads), w = (int)(id / c.heads);
+    const int64_t id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (id >= (int64_t)p.max_items * c.heads * 2) return;
+    const int which = (int)(id & 1), h = (int)((id >> 1) % c.heads), w = (int)((id >> 1) / c.heads);
     const int r = p.items[2 * (int64_t)w], j = p.items[2 * (int64_t)w + 1];
     if (r < 0 || r >= c.requests || j < 0 || j >= c.width) return;
     const Span s = request_span(p.cu_tokens, c.len, r, p.max_tokens, c.width);
+    const int blk = c.table[(int64_t)r * c.width + j];
     const int first = s.before >= 0 ? s.before / kKvBlock : 0;
-    const int64_t row0 = ((int64_t)r * c.heads + h) * kKvBlock;  // the tail's first row
+    const int64_t x_tok = which ? p.v_tok : p.k_tok;
+    const uint16_t* const x = (which ? p.v : p.k) + h * D + E * cl;
+    uint16_t* const tail = (which ? c.v_tail : c.k_tail) + ((int64_t)r * c.heads + h) * kKvBlock * D + E * cl;
 
-    // Row t of block jb, from the new tokens or (`old`) from the tail; 0 for rows that are neither.
-    auto load = [&](const uint16_t* x, int64_t x_tok, const uint16_t* tail, int jb, int t) {
-        const int pos = jb * kKvBlock + t;
-        piece v = {};
-        if (pos >= s.total) return v;
-        if (pos >= s.before)
-            v = *reinterpret_cast<const piece*>(x + (s.t0 + (int64_t)(pos - s.before)) * x_tok + h * D + E * cl);
-        else
-            v = *reinterpret_cast<const piece*>(tail + (row0 + t) * D + E * cl);
-        return v;
+    auto fresh = [&](int pos) {  // the new token at position pos
+        return *reinterpret_cast<const piece*>(x + (s.t0 + (int64_t)(pos - s.before)) * x_tok);
     };
     auto to_tail = [&](int jb) {  // the new tokens of the partial block jb
-#pragma unroll 4
-        for (int i = 0; i < 16; i++) {
-            const int t = 16 * (i >> 2) + 4 * g + (i & 3), pos = jb * kKvBlock + t;
-            if (pos < s.before || pos >= s.total) continue;
-            const piece a = load(p.k, p.k_tok, nullptr, jb, t), b = load(p.v, p.v_tok, nullptr, jb, t);
-            *reinterpret_cast<piece*>(c.k_tail + (row0 + t) * D + E * cl) = a;
-            *reinterpret_cast<piece*>(c.v_tail + (row0 + t) * D + E * cl) = b;
-        }
+        const int lo = max(s.before - jb * kKvBlock, 0), hi = s.total - jb * kKvBlock;
+        for (int t = lo + g; t < hi; t += 4) *reinterpret_cast<piece*>(tail + t * D) = fresh(jb * kKvBlock + t);
     };
     // The tail holds the first block's old tokens until that block's wave has read them: where the step both
     // completes that block and leaves a new tail, that wave writes the tail, after its loads.
@@ -327,63 +316,57 @@ __global__ __launch_bounds__(256) void kv8_append(Kv8Append p) {
         if (j * kKvBlock < s.total && (j == first || !old_tail)) to_tail(j);
         return;
     }
-    const int blk = c.table[(int64_t)r * c.width + j];
-    const bool in_pool = blk >= 0 && blk < c.blocks;
+    piece d[16];
 #pragma unroll
-    for (int which = 0; which < 2; which++) {
-        const uint16_t* x = which ? p.v : p.k;
-        const int64_t x_tok = which ? p.v_tok : p.k_tok;
-        const uint16_t* tail = which ? c.v_tail : c.k_tail;
-        piece d[16];
+    for (int i = 0; i < 16; i++) {
+        const int t = 16 * (i >> 2) + 4 * g + (i & 3), pos = j * kKvBlock + t;
+        d[i] = pos >= s.before ? fresh(pos) : *reinterpret_cast<const piece*>(tail + t * D);
+    }
+    float amax = 0.f;
+    bool bad = false;
 #pragma unroll
-        for (int i = 0; i < 16; i++) d[i] = load(x, x_tok, tail, j, 16 * (i >> 2) + 4 * g + (i & 3));
-        float amax = 0.f;
-        bool bad = false;
+    for (int i = 0; i < 16; i++)
 #pragma unroll
-        for (int i = 0; i < 16; i++)
+        for (int e = 0; e < W; e++) {
+            // largest magnitude, and whether one is a NaN or an infinity (all bits of the exponent set)
+            constexpr uint32_t ex = BF16 ? 0x7f80u : 0x7c00u;
+            const uint32_t u = d[i][e];
+            bad |= (u & ex) == ex || ((u >> 16) & ex) == ex;
+            amax = fmaxf(amax, fmaxf(fabsf(half_to_f32<BF16>(u & 0xffffu)), fabsf(half_to_f32<BF16>(u >> 16))));
+        }
 #pragma unroll
-            for (int e = 0; e < W; e++) {
-                // largest magnitude, and whether one is a NaN or an infinity (all bits of the exponent set)
-                constexpr uint32_t ex = BF16 ? 0x7f80u : 0x7c00u;
-                const uint32_t u = d[i][e];
-                bad |= (u & ex) == ex || ((u >> 16) & ex) == ex;
-                amax = fmaxf(amax, fmaxf(fabsf(half_to_f32<BF16>(u & 0xffffu)), fabsf(half_to_f32<BF16>(u >> 16))));
+    for (int o = 32; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+    bad = __ballot(bad) != 0;
+    float scale, mul;
+    block_scale<CODE>(bad ? 0.f : amax, scale, mul);
+    if (blk >= 0 && blk < c.blocks) {
+        const int64_t at = (int64_t)blk * c.heads + h;
+        if (lane == 0) c.scales[2 * at + which] = bad ? __builtin_nanf("") : scale;
+        uint8_t* const out = (which ? c.v : c.k) + at * kKvBlock * D;
+        auto val = [&](int i, int e) {
+            const uint32_t u = d[i][e >> 1];
+            const float f = half_to_f32<BF16>((e & 1) ? u >> 16 : u & 0xffffu) * mul;
+            return bad ? 0.f : f;
+        };
+        if (which == 0) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int t = 16 * (i >> 2) + 4 * g + (i & 3);
+                uint32_t* dst = reinterpret_cast<uint32_t*>(out + t * D + E * cl);
+                const uint32_t w0 = encode4<CODE>(val(i, 0), val(i, 1), val(i, 2), val(i, 3));
+                if constexpr (E == 4) *dst = w0;
+                else
+                    *reinterpret_cast<u32x2*>(dst) =
+                        u32x2{w0, encode4<CODE>(val(i, E - 4), val(i, E - 3), val(i, E - 2), val(i, E - 1))};
             }
+        } else {
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
-        bad = __ballot(bad) != 0;
-        float scale, mul;
-        block_scale<CODE>(bad ? 0.f : amax, scale, mul);
-        if (bad) scale = __builtin_nanf("");
-        if (in_pool) {
-            const int64_t at = ((int64_t)blk * c.heads + h);
-            if (lane == 0) c.scales[2 * at + which] = scale;
-            uint8_t* out = (which ? c.v : c.k) + at * kKvBlock * D;
-            auto val = [&](int i, int e) {
-                const uint32_t u = d[i][e >> 1];
-                const float f = half_to_f32<BF16>((e & 1) ? u >> 16 : u & 0xffffu) * mul;
-                return bad ? 0.f : f;
-            };
-            if (which == 0) {
+            for (int e = 0; e < E; e++) {
+                u32x4 word;  // words (c, a): tokens 32 c + 16 a + 4 g + 0..3
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int t = 16 * (i >> 2) + 4 * g + (i & 3);
-                    uint32_t* dst = reinterpret_cast<uint32_t*>(out + t * D + E * cl);
-                    const uint32_t w0 = encode4<CODE>(val(i, 0), val(i, 1), val(i, 2), val(i, 3));
-                    if constexpr (E == 4) *dst = w0;
-                    else
-                        *reinterpret_cast<u32x2*>(dst) =
-                            u32x2{w0, encode4<CODE>(val(i, E - 4), val(i, E - 3), val(i, E - 2), val(i, E - 1))};
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; e++) {
-                    u32x4 word;  // words (c, a): tokens 32 c + 16 a + 4 g + 0..3
-#pragma unroll
-                    for (int q = 0; q < 4; q++)
-                        word[q] = encode4<CODE>(val(4 * q, e), val(4 * q + 1, e), val(4 * q + 2, e), val(4 * q + 3, e));
-                    *reinterpret_cast<u32x4*>(out + (E * cl + e) * kKvBlock + 16 * g) = word;
-                }
+                for (int q = 0; q < 4; q++)
+                    word[q] = encode4<CODE>(val(4 * q, e), val(4 * q + 1, e), val(4 * q + 2, e), val(4 * q + 3, e));
+                *reinterpret_cast<u32x4*>(out + (E * cl + e) * kKvBlock + 16 * g) = word;
             }
         }
     }
@@ -392,7 +375,7 @@ __global__ __launch_bounds__(256) void kv8_append(Kv8Append p) {
 
 template <int CODE, bool BF16>
 hipError_t append_d(const Kv8Append& p, int head_dim, hipStream_t s) {
-    const int64_t waves = (int64_t)p.max_items * p.c.heads, grid = (waves + 3) / 4;
+    const int64_t waves = (int64_t)p.max_items * p.c.heads * 2, grid = (waves + 3) / 4;
     if (grid <= 0 || grid > 0x7fffffff) return hipErrorInvalidValue;
     if (head_dim == 64) hipLaunchKernelGGL((kv8_append<CODE, BF16, 64>), dim3((unsigned)grid), dim3(256), 0, s, p);
     else hipLaunchKernelGGL((kv8_append<CODE, BF16, 128>), dim3((unsigned)grid), dim3(256), 0, s, p);

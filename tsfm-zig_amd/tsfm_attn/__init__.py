@@ -188,6 +188,7 @@ assert _ATTN_PACK.size == ctypes.sizeof(AttnArgs)
 
 
 _lib: Optional[ctypes.CDLL] = None
+_raw_current: Any = None  # torch's current raw stream of a device, once load() has found torch
 
 
 class VariateArgs(ctypes.Structure):
@@ -470,8 +471,11 @@ def load(path: Optional[os.PathLike] = None) -> ctypes.CDLL:
     # system runtime loaded first (by this library) would not satisfy them and torch would load a
     # second one, under which it sees no device and its streams mean nothing to this library.
     # Loading torch first lets this library's libamdhip64.so.7 dependency bind to torch's copy.
+    global _raw_current
     try:
         import torch  # noqa: F401
+
+        _raw_current = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     except ImportError:
         pass
     lib = ctypes.CDLL(str(p))
@@ -594,6 +598,13 @@ def _dtype_code(x: Any) -> int:
         raise TypeError(f"unsupported element type {name}")
     _DTYPE_CODES[dt] = code
     return code
+
+
+def _raw_stream(x: Any, stream: Any) -> int:
+    """``_stream_of`` for a device tensor, without the lookups that a small call would feel."""
+    if stream is None and _raw_current is not None:
+        return _raw_current(x.get_device())
+    return _stream_of(x, stream) or 0
 
 
 def _stream_of(x: Any, stream: Any) -> Optional[int]:
@@ -1266,20 +1277,49 @@ _F8_QUANTIZE_PACK = _packer(F8QuantizeArgs)
 _F8_GEMM_PACK = _packer(F8GemmArgs)
 
 
+class _Types:
+    """torch's dtypes, looked up once (a comparison by name costs more than a small call's other checks)."""
+
+    def __init__(self):
+        import torch
+
+        self.i32, self.i64, self.f32, self.i8, self.e4m3 = (torch.int32, torch.int64, torch.float32, torch.int8,
+                                                            torch.float8_e4m3fn)
+
+
+_types_once: Optional[_Types] = None
+
+
+def _types() -> _Types:
+    global _types_once
+    if _types_once is None:
+        _types_once = _Types()
+    return _types_once
+
+
 def _want(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
 
 
+def _plain(tensors: Sequence[Any], dtype: Any) -> bool:
+    """Whether all are contiguous tensors of `dtype` on a GPU."""
+    for t in tensors:
+        if t.dtype is not dtype or not t.is_cuda or not t.is_contiguous():
+            return False
+    return True
+
+
 def _rows_of(x: Any, what: str, width: int) -> int:
-    """The row stride of a tensor of rows of `width` elements, (rows, width) or (rows, heads, head_dim)."""
-    if x.dim() == 3:
-        _want(x.shape[1] * x.shape[2] == width and x.stride(2) == 1 and (x.stride(1) == x.shape[2] or x.shape[1] == 1),
-              f"{what}: rows of {width} consecutive elements")
+    """The row stride of a GPU tensor of rows of `width` elements, (rows, width) or (rows, heads, head_dim)."""
+    shape, step = x.shape, x.stride()
+    if len(shape) == 3:
+        ok = shape[1] * shape[2] == width and step[2] == 1 and (step[1] == shape[2] or shape[1] == 1)
     else:
-        _want(x.dim() == 2 and x.shape[1] == width and (x.stride(1) == 1 or width == 1),
-              f"{what}: rows of {width} consecutive elements")
-    return x.stride(0)
+        ok = len(shape) == 2 and shape[1] == width and (step[1] == 1 or width == 1)
+    if not (ok and x.is_cuda):
+        raise ValueError(f"{what}: a GPU tensor of rows of {width} consecutive elements")
+    return step[0]
 
 
 def _kv8_items(requests: int, tokens: int) -> int:
@@ -1294,16 +1334,17 @@ class Kv8Cache:
     (requests, blocks of a request) and ``length`` (requests) int32."""
 
     def __init__(self, k, v, scales, k_tail, v_tail, table, length):
+        ty = _types()
         blocks, kv_heads, _, head_dim = k.shape
         requests = length.shape[0]
-        code = {"torch.float8_e4m3fn": CODE_E4M3, "torch.int8": CODE_I8}.get(str(k.dtype))
+        code = {ty.e4m3: CODE_E4M3, ty.i8: CODE_I8}.get(k.dtype)
         _want(code is not None and v.dtype == k.dtype, "k and v: torch.float8_e4m3fn or torch.int8")
         _want(k.shape[2] == KV8_BLOCK and tuple(v.shape) == (blocks, kv_heads, head_dim, KV8_BLOCK), "k or v: shape")
-        _want(tuple(scales.shape) == (blocks, kv_heads, 2) and str(scales.dtype) == "torch.float32", "scales")
+        _want(tuple(scales.shape) == (blocks, kv_heads, 2) and scales.dtype == ty.f32, "scales: (blocks, kv heads, 2) f32")
         tail = (requests, kv_heads, KV8_BLOCK, head_dim)
         _want(tuple(k_tail.shape) == tail and tuple(v_tail.shape) == tail and k_tail.dtype == v_tail.dtype, "tails")
         _want(table.dim() == 2 and table.shape[0] == requests, "table: (requests, blocks of a request)")
-        _want(str(table.dtype) == str(length.dtype) == "torch.int32", "table and length: int32")
+        _want(table.dtype == length.dtype == ty.i32, "table and length: int32")
         parts = (k, v, scales, k_tail, v_tail, table, length)
         _want(all(t.is_cuda and t.is_contiguous() and t.device == k.device for t in parts),
               "the cache's tensors: contiguous, on one GPU")
@@ -1318,48 +1359,47 @@ def kv8_plan(n_new, length, length_out, free_list, free_count, free_count_out, t
              slots, pos, items, status, stream=None) -> int:
     """``tsfm_kv8_plan``: block tables and slot maps from the requests' new token counts. All int32 but ``slots``
     (int64); ``length_out`` may be ``length`` and ``free_count_out`` ``free_count``."""
+    ty = _types()
     r = n_new.shape[0]
-    ints = (n_new, length, length_out, free_list, free_count, free_count_out, table, cu_tokens, cu_blocks, cu_items,
-            pos, items, status)
-    _want(all(str(t.dtype) == "torch.int32" for t in ints) and str(slots.dtype) == "torch.int64", "int32, slots int64")
-    _want(all(t.is_cuda and t.is_contiguous() for t in ints) and slots.is_cuda and slots.is_contiguous(),
-          "contiguous tensors on the GPU")
-    _want(length.shape[0] == length_out.shape[0] == table.shape[0] == r, "one entry per request")
-    _want(cu_tokens.shape[0] == cu_blocks.shape[0] == cu_items.shape[0] == r + 1, "prefix sums: requests + 1 entries")
-    _want(pos.shape[0] == slots.shape[0] and items.shape[1] == 2 and status.numel() >= 4, "slots, pos, items, status")
-    args = _KV8_PLAN_PACK.pack(r, free_list.shape[0], table.shape[1], slots.shape[0], items.shape[0], DEVICE_PTRS,
+    room = slots.shape[0]
+    if not (_plain((n_new, length, length_out, free_list, free_count, free_count_out, table, cu_tokens, cu_blocks,
+                    cu_items, pos, items, status), ty.i32) and _plain((slots,), ty.i64)):
+        raise ValueError("the plan's tensors: contiguous int32 (slots int64) on the GPU")
+    if not (length.shape[0] == length_out.shape[0] == table.shape[0] == r and pos.shape[0] == room
+            and cu_tokens.shape[0] == cu_blocks.shape[0] == cu_items.shape[0] == r + 1 and items.shape[1] == 2
+            and status.shape[0] >= 4):
+        raise ValueError("the plan's tensors: one entry per request (prefix sums one more), per token, per item")
+    args = _KV8_PLAN_PACK.pack(r, free_list.shape[0], table.shape[1], room, items.shape[0], DEVICE_PTRS,
                                n_new.data_ptr(), length.data_ptr(), length_out.data_ptr(), free_list.data_ptr(),
                                free_count.data_ptr(), free_count_out.data_ptr(), table.data_ptr(),
                                cu_tokens.data_ptr(), cu_blocks.data_ptr(), cu_items.data_ptr(), slots.data_ptr(),
-                               pos.data_ptr(), items.data_ptr(), status.data_ptr(), _stream_of(n_new, stream) or 0)
-    return int(load().tsfm_kv8_plan(args))
+                               pos.data_ptr(), items.data_ptr(), status.data_ptr(), _raw_stream(n_new, stream))
+    return load().tsfm_kv8_plan(args)
 
 
 def kv8_release(drop, length, table, free_list, free_count, status, stream=None) -> int:
     """``tsfm_kv8_release``: ends the requests whose ``drop`` (uint8 or bool) is not 0."""
-    ints = (length, table, free_list, free_count, status)
-    _want(all(str(t.dtype) == "torch.int32" for t in ints) and drop.element_size() == 1, "int32, drop of bytes")
-    _want(all(t.is_cuda and t.is_contiguous() for t in (*ints, drop)), "contiguous tensors on the GPU")
+    _want(_plain((length, table, free_list, free_count, status), _types().i32), "contiguous int32 tensors on the GPU")
+    _want(drop.element_size() == 1 and drop.is_cuda and drop.is_contiguous(), "drop: contiguous bytes on the GPU")
     _want(drop.shape[0] == length.shape[0] == table.shape[0] and status.numel() >= 2, "one entry per request")
     args = _KV8_RELEASE_PACK.pack(length.shape[0], free_list.shape[0], table.shape[1], DEVICE_PTRS, drop.data_ptr(),
                                   length.data_ptr(), table.data_ptr(), free_list.data_ptr(), free_count.data_ptr(),
-                                  status.data_ptr(), _stream_of(length, stream) or 0)
-    return int(load().tsfm_kv8_release(args))
+                                  status.data_ptr(), _raw_stream(length, stream))
+    return load().tsfm_kv8_release(args)
 
 
 def kv8_append(cache: Kv8Cache, k, v, cu_tokens, items, stream=None) -> int:
     """``tsfm_kv8_append``: the K/V of the step's packed tokens, (tokens, kv heads * head dim) rows of any stride, into
     the cache. ``cu_tokens`` and ``items`` are ``kv8_plan``'s."""
-    _want(k.dtype == v.dtype == cache.dtype and k.shape[0] == v.shape[0], "k and v: the cache's dtype, a row per token")
-    _want(k.is_cuda and v.is_cuda and cu_tokens.is_cuda and items.is_cuda and items.is_contiguous()
-          and cu_tokens.is_contiguous(), "tensors on the GPU")
-    _want(str(cu_tokens.dtype) == str(items.dtype) == "torch.int32" and cu_tokens.shape[0] == cache.requests + 1,
-          "cu_tokens and items: int32, as planned")
-    width = cache.kv_heads * cache.head_dim
-    args = _KV8_APPEND_PACK.pack(*cache._fields, k.shape[0], items.shape[0], DEVICE_PTRS, cu_tokens.data_ptr(),
+    tokens, width = k.shape[0], cache.kv_heads * cache.head_dim
+    if not (k.dtype is cache.dtype and v.dtype is cache.dtype and v.shape[0] == tokens):
+        raise ValueError("k and v: the cache's dtype, a row per token")
+    if not (_plain((cu_tokens, items), _types().i32) and cu_tokens.shape[0] == cache.requests + 1 and items.shape[1] == 2):
+        raise ValueError("cu_tokens and items: as planned")
+    args = _KV8_APPEND_PACK.pack(*cache._fields, tokens, items.shape[0], DEVICE_PTRS, cu_tokens.data_ptr(),
                                  items.data_ptr(), k.data_ptr(), _rows_of(k, "k", width), v.data_ptr(),
-                                 _rows_of(v, "v", width), _stream_of(k, stream) or 0)
-    return int(load().tsfm_kv8_append(args))
+                                 _rows_of(v, "v", width), _raw_stream(k, stream))
+    return load().tsfm_kv8_append(args)
 
 
 def _kv8_attend_sizes(cache: Kv8Cache, heads: int, tokens: int, max_new: int, max_len: int, scale: float) -> tuple:
@@ -1370,7 +1410,7 @@ def kv8_attend_workspace(cache: Kv8Cache, heads: int, tokens: int, max_new: int 
                          stream=None) -> int:
     """``tsfm_kv8_attend_workspace``: bytes of workspace that ``kv8_attend`` with these sizes needs."""
     args = _KV8_ATTEND_PACK.pack(*_kv8_attend_sizes(cache, heads, tokens, max_new, max_len, 0.0), 0, 0, 0, 0, 0, 0, 0,
-                                 _stream_of(cache.k, stream) or 0)
+                                 _raw_stream(cache.k, stream))
     n = int(load().tsfm_kv8_attend_workspace(args))
     if n < 0:
         raise TsfmError(E_UNSUPPORTED, last_error())
@@ -1381,17 +1421,20 @@ def kv8_attend(cache: Kv8Cache, q, o, cu_tokens, *, scale: float, max_new: int =
                stream=None) -> int:
     """``tsfm_kv8_attend``: causal attention of the step's packed queries, (tokens, heads, head dim) or (tokens,
     heads * head dim), over the cache, into ``o`` of the same shape."""
-    width = q.shape[1] * q.shape[2] if q.dim() == 3 else q.shape[1]
-    _want(q.dtype == o.dtype == cache.dtype and o.shape == q.shape, "q and o: the cache's dtype, one shape")
-    _want(q.is_cuda and o.is_cuda and cu_tokens.is_cuda and cu_tokens.is_contiguous(), "tensors on the GPU")
-    _want(str(cu_tokens.dtype) == "torch.int32" and cu_tokens.shape[0] == cache.requests + 1, "cu_tokens: as planned")
-    _want(width % cache.head_dim == 0, "q: whole heads")
-    room = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    args = _KV8_ATTEND_PACK.pack(*_kv8_attend_sizes(cache, width // cache.head_dim, q.shape[0], max_new, max_len, scale),
+    shape, dt = q.shape, cache.dtype
+    width = shape[1] * shape[2] if len(shape) == 3 else shape[1]
+    if not (q.dtype is dt and o.dtype is dt and o.shape == shape and width % cache.head_dim == 0):
+        raise ValueError("q and o: the cache's dtype, one shape of whole heads")
+    if not (_plain((cu_tokens,), _types().i32) and cu_tokens.shape[0] == cache.requests + 1):
+        raise ValueError("cu_tokens: as planned")
+    at, room = 0, 0
+    if workspace is not None:
+        _want(workspace.is_cuda and workspace.is_contiguous(), "workspace: contiguous, on the GPU")
+        at, room = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    args = _KV8_ATTEND_PACK.pack(*cache._fields, width // cache.head_dim, shape[0], max_new, max_len, scale, DEVICE_PTRS,
                                  cu_tokens.data_ptr(), q.data_ptr(), _rows_of(q, "q", width), o.data_ptr(),
-                                 _rows_of(o, "o", width), 0 if workspace is None else workspace.data_ptr(), room,
-                                 _stream_of(q, stream) or 0)
-    return int(load().tsfm_kv8_attend(args))
+                                 _rows_of(o, "o", width), at, room, _raw_stream(q, stream))
+    return load().tsfm_kv8_attend(args)
 
 
 class Kv8Pool:
@@ -1463,32 +1506,34 @@ class Kv8Pool:
 def f8_quantize(x, codes, scales, group_rows: int = 1, stream=None) -> int:
     """``tsfm_f8_quantize``: ``x`` (rows, cols) f32, bf16 or f16 to e4m3 ``codes`` and f32 ``scales`` (ceil(rows /
     group_rows), ceil(cols / 128)): group_rows 1 for activations, 128 for weights."""
+    ty = _types()
     rows, cols = x.shape
-    groups, scale_rows = -(-cols // 128), -(-rows // group_rows)
-    _want(x.is_cuda and codes.is_cuda and scales.is_cuda, "tensors on the GPU")
-    _want(codes.shape == x.shape and str(codes.dtype) == "torch.float8_e4m3fn", "codes: torch.float8_e4m3fn as x")
-    _want(tuple(scales.shape) == (scale_rows, groups) and str(scales.dtype) == "torch.float32", "scales: f32 per group")
+    groups = -(-cols // 128)
+    if not (codes.shape == x.shape and codes.dtype is ty.e4m3):
+        raise ValueError("codes: torch.float8_e4m3fn in x's shape")
+    if not (scales.dtype is ty.f32 and scales.shape[0] == (rows if group_rows == 1 else -(-rows // group_rows))):
+        raise ValueError("scales: f32, one row per group of rows")
     args = _F8_QUANTIZE_PACK.pack(_dtype_code(x), rows, cols, group_rows, DEVICE_PTRS, x.data_ptr(),
                                   _rows_of(x, "x", cols), codes.data_ptr(), _rows_of(codes, "codes", cols),
-                                  scales.data_ptr(), _rows_of(scales, "scales", groups), _stream_of(x, stream) or 0)
-    return int(load().tsfm_f8_quantize(args))
+                                  scales.data_ptr(), _rows_of(scales, "scales", groups), _raw_stream(x, stream))
+    return load().tsfm_f8_quantize(args)
 
 
 def f8_gemm_nt(a, a_scales, b, b_scales, c, stream=None) -> int:
     """``tsfm_f8_gemm_nt``: c (m, n) = a (m, k) b (n, k)^T of e4m3 codes with scales (m, ceil(k / 128)) and (ceil(n /
     128), ceil(k / 128)); c f32, bf16 or f16."""
+    ty = _types()
     (m, k), n = a.shape, b.shape[0]
-    kb, nb = -(-k // 128), -(-n // 128)
-    _want(all(t.is_cuda for t in (a, a_scales, b, b_scales, c)), "tensors on the GPU")
-    _want(str(a.dtype) == str(b.dtype) == "torch.float8_e4m3fn" and b.shape[1] == k, "a and b: e4m3 codes of one k")
-    _want(tuple(a_scales.shape) == (m, kb) and tuple(b_scales.shape) == (nb, kb)
-          and str(a_scales.dtype) == str(b_scales.dtype) == "torch.float32", "scales: f32 per group")
-    _want(tuple(c.shape) == (m, n), "c: (m, n)")
+    kb = -(-k // 128)
+    if not (a.dtype is ty.e4m3 and b.dtype is ty.e4m3 and a_scales.dtype is ty.f32 and b_scales.dtype is ty.f32):
+        raise ValueError("a and b: torch.float8_e4m3fn, their scales f32")
+    if not (a_scales.shape[0] == m and b_scales.shape[0] == -(-n // 128) and c.shape[0] == m):
+        raise ValueError("a_scales: (m, ceil(k / 128)); b_scales: (ceil(n / 128), ceil(k / 128)); c: (m, n)")
     args = _F8_GEMM_PACK.pack(m, n, k, _dtype_code(c), DEVICE_PTRS, a.data_ptr(), _rows_of(a, "a", k),
                               a_scales.data_ptr(), _rows_of(a_scales, "a_scales", kb), b.data_ptr(),
                               _rows_of(b, "b", k), b_scales.data_ptr(), _rows_of(b_scales, "b_scales", kb),
-                              c.data_ptr(), _rows_of(c, "c", n), _stream_of(a, stream) or 0)
-    return int(load().tsfm_f8_gemm_nt(args))
+                              c.data_ptr(), _rows_of(c, "c", n), _raw_stream(a, stream))
+    return load().tsfm_f8_gemm_nt(args)
 
 
 # ---- Timestral forecast -------------------------------------------------------------------------
