@@ -400,6 +400,289 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(few_wav
     }
 }
 
+// ---- many rows: tiles through LDS ----
+// One workgroup = (request, K/V head, 128 rows, chunk of the keys), four waves of 32 rows on v_mfma_f32_32x32x16. Each
+// cache block is decoded once per workgroup, into LDS in the instructions' operand order, while the waves compute the
+// block before it; its codes are loaded a block earlier still. Lane l of a score block holds one row (l % 32) and keys
+// 8 (i / 4) + 4 (l / 32) + i % 4, i < 16: the order in which V's operand takes them, so the weights go from the scores'
+// registers straight into the second product. Bound by the matrix and vector units together.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <bool BF16>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (BF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+constexpr int MW = 4;          // waves
+constexpr int MROWS = 32 * MW;  // rows of a workgroup
+// The running max follows a block's only when it is passed by this much (exp2 units): weights up to 2^8 cost nothing,
+// and O is rescaled a few times per row instead of in every block.
+constexpr float kSlack = 8.f;
+
+template <int CODE, bool BF16, int D>
+__global__ __launch_bounds__(64 * MW) __attribute__((amdgpu_waves_per_eu(2, 2))) void attend_many(Kv8Attend p) {
+    constexpr int KS = D / 16;  // 16-dim steps of a score
+    constexpr int DB = D / 32;  // 32-dim blocks of O
+    constexpr int U = D / 64;   // 16-byte pieces of K, and of V, per thread and block
+    // Operand blocks of 1 KB (lane l's 16 bytes at 16 l). K: (32 keys, 16-dim step); V: (16 keys, 32 dims).
+    constexpr uint32_t kOp = 1024 + 128;  // 128 bytes apart: a staging wave's pieces of two steps lie on different banks
+    constexpr uint32_t kK = 2 * KS * kOp, kStage = kK + 4 * DB * kOp;
+    __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+    __shared__ unsigned long long bad_keys;
+    typedef __attribute__((address_space(3))) u32x4* lds_u32x4_ptr;
+    typedef __attribute__((address_space(3))) u32x2* lds_u32x2_ptr;
+    typedef __attribute__((address_space(3))) uint16_t* lds_u16_ptr;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lq = lane & 31, lh = lane >> 5;
+    const Kv8& c = p.c;
+    // Row tiles of one (request, head, chunk) read the same keys: on one XCD, whose L2 then holds them. Workgroups go to
+    // the 8 XCDs in turn, and the triples are dealt to XCDs in turn too, heads first: every XCD has its share of each
+    // request, however their lengths differ (requests dealt to XCDs whole: 999 us where this takes 480). Late tiles,
+    // which read the most keys, first.
+    const int idx = blockIdx.x >> 3;
+    const int tile0 = p.tiles - 1 - idx % p.tiles;
+    int id = idx / p.tiles * 8 + (blockIdx.x & 7);
+    const int h = id % c.heads;
+    id /= c.heads;
+    const int r = id % c.requests, ck = id / c.requests;
+    if (ck >= p.chunks) return;
+    const Span s = request_span(p.cu_tokens, c.len, r, p.max_tokens, c.width);
+    const int G = p.group;
+    const int64_t rows = (int64_t)s.n * G;
+    const int nfull = s.total / kKvBlock;
+    const int32_t* __restrict__ table = c.table + (int64_t)r * c.width;
+
+    for (int64_t row0 = (int64_t)tile0 * MROWS; row0 < rows; row0 += (int64_t)p.tiles * MROWS) {
+        const int last = (int)((min(rows, row0 + MROWS) - 1) / G);
+        const int kend = keys_to(s, last), nblk = (kend + kKvBlock - 1) / kKvBlock;
+        const int cb = chunk_blocks(p, nblk), nchunk = max(1, (nblk + cb - 1) / cb);
+        if (ck >= nchunk) continue;
+        const int b0 = ck * cb, b1 = min(nblk, b0 + cb);
+        const int bq = min(b1, nfull);  // end of the chunk's whole blocks
+
+        // ---- this wave's rows ----
+        const int64_t wrow = row0 + 32 * wave, row = wrow + lq;
+        const int tok = (int)(min(row, rows - 1) / G), hq = h * G + (int)(min(row, rows - 1) % G);
+        const int kv_end = row < rows ? keys_to(s, tok) : 0;                                        // keys of the lane's row
+        const int plain_end = wrow < rows ? keys_to(s, (int)(wrow / G)) : 0;                        // of all the wave's rows
+        const int wave_end = wrow < rows ? keys_to(s, (int)((min(rows, wrow + 32) - 1) / G)) : 0;  // of any
+        u32x4 qf[KS];
+#pragma unroll
+        for (int t = 0; t < KS; t++)
+            qf[t] = row < rows ? ld16(p.q + (s.t0 + (int64_t)tok) * p.q_tok + hq * D + 16 * t + 8 * lh) : u32x4{0, 0, 0, 0};
+        f32x16 oacc[DB];
+#pragma unroll
+        for (int db = 0; db < DB; db++) oacc[db] = f32x16{};
+        float m_run = kNegInf, l_run = 0.f;
+
+        // ---- staging ----
+        // K: a wave's load covers 1 KB: 16 keys of 64 dims (lane: key l % 16, step l / 16) or 8 keys of 128 (key l % 8,
+        // step l / 8). V: the thread's dim and 16-byte piece g of its tokens.
+        u32x4 kc[U], vc[U];
+        auto load = [&](int blk) {
+            const bool ok = blk >= 0 && blk < c.blocks;
+            const int64_t at = ((int64_t)(ok ? blk : 0) * c.heads + h) * kKvBlock * D;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int key = U == 1 ? 16 * wave + (lane & 15) : 16 * wave + 8 * u + (lane & 7);
+                const int step = U == 1 ? lane >> 4 : lane >> 3;
+                kc[u] = ld16(c.k + at + key * D + 16 * step);
+                const int dim = 16 * wave + 64 * u + (lane & 15);
+                vc[u] = ld16(c.v + at + dim * kKvBlock + 16 * (lane >> 4));
+            }
+        };
+        auto stage = [&](int buf) {
+            const uint32_t st = lds0 + buf * kStage;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int key = U == 1 ? 16 * wave + (lane & 15) : 16 * wave + 8 * u + (lane & 7);
+                const int step = U == 1 ? lane >> 4 : lane >> 3;
+                const uint32_t a = st + ((key >> 5) * KS + step) * kOp + 16 * (key & 31);
+                *(lds_u32x4_ptr)(uintptr_t)a = decode8<CODE, BF16>(kc[u][0], kc[u][1]);
+                *(lds_u32x4_ptr)(uintptr_t)(a + 512) = decode8<CODE, BF16>(kc[u][2], kc[u][3]);
+                // V: words (c2, a2) of piece g are tokens 16 (2 c2 + a2) + 4 g .. + 3: four of the operand's eight slots
+                const int dim = 16 * wave + 64 * u + (lane & 15), g = lane >> 4;
+                const uint32_t b = st + kK + (dim >> 5) * kOp + 16 * (32 * (g & 1) + (dim & 31)) + 8 * (g >> 1);
+                const u32x4 lo = decode8<CODE, BF16>(vc[u][0], vc[u][1]), hi = decode8<CODE, BF16>(vc[u][2], vc[u][3]);
+                *(lds_u32x2_ptr)(uintptr_t)(b) = u32x2{lo[0], lo[1]};
+                *(lds_u32x2_ptr)(uintptr_t)(b + DB * kOp) = u32x2{lo[2], lo[3]};
+                *(lds_u32x2_ptr)(uintptr_t)(b + 2 * DB * kOp) = u32x2{hi[0], hi[1]};
+                *(lds_u32x2_ptr)(uintptr_t)(b + 3 * DB * kOp) = u32x2{hi[2], hi[3]};
+            }
+        };
+        // The tail's values as they are; rows past the last token 0. V's that are no numbers: 0, and their keys noted.
+        auto stage_tail = [&](int buf) {
+            int tid_t = tid;  // opaque: its addresses are not kept across the loop
+            asm volatile("" : "+v"(tid_t));
+            const uint32_t st = lds0 + buf * kStage;
+            const int live = s.total - nfull * kKvBlock;
+            const int64_t at = ((int64_t)r * c.heads + h) * kKvBlock * D;
+#pragma unroll 1
+            for (int i = tid_t; i < kKvBlock * D / 8; i += 64 * MW) {
+                const int key = i / (D / 8), d0 = 8 * (i % (D / 8));
+                const u32x4 z = {0, 0, 0, 0};
+                const u32x4 x = key < live ? ld16(c.k_tail + at + key * D + d0) : z;
+                *(lds_u32x4_ptr)(uintptr_t)(st + ((key >> 5) * KS + (d0 >> 4)) * kOp + 16 * (32 * ((d0 >> 3) & 1) + (key & 31))) = x;
+                const u32x4 y = key < live ? ld16(c.v_tail + at + key * D + d0) : z;
+                const int slot = key & 15;  // of its 16 keys: lane half (slot / 4) % 2, element 4 (slot / 8) + slot % 4
+                const uint32_t b = st + kK + ((key >> 4) * DB + (d0 >> 5)) * kOp + 16 * (32 * ((slot >> 2) & 1) + (d0 & 31)) +
+                                   2 * (4 * (slot >> 3) + (slot & 3));
+                bool any = false;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    constexpr uint32_t ex = BF16 ? 0x7f80u : 0x7c00u;
+                    uint32_t v = (e & 1) ? y[e >> 1] >> 16 : y[e >> 1] & 0xffffu;
+                    if ((v & ex) == ex) {
+                        any = true;
+                        v = 0;
+                    }
+                    *(lds_u16_ptr)(uintptr_t)(b + 16 * e) = (uint16_t)v;
+                }
+                if (any) atomicOr(&bad_keys, 1ull << key);
+            }
+        };
+
+        // ---- one block ----
+        auto compute = [&](int j, int buf, float kx, float lv, bool tail) {
+            const int k0 = j * kKvBlock;
+            if (k0 >= wave_end) return;
+            const float inv_v = __builtin_amdgcn_exp2f(-lv);
+            const uint32_t st = lds0 + buf * kStage + 16 * lane;
+            f32x16 sb[2] = {f32x16{}, f32x16{}};
+#pragma unroll
+            for (int t = 0; t < KS; t++)  // two independent chains: an instruction's result is twice its issue away
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++)
+                    sb[kb] = mfma32<BF16>(*(lds_u32x4_ptr)(uintptr_t)(st + (kb * KS + t) * kOp), qf[t], sb[kb]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (k0 + kKvBlock > plain_end) {
+                const int rel = kv_end - k0 - 4 * lh;  // register i's key is seen where its offset is below
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float t = __builtin_fmaf(sb[kb][i], kx, lv);
+                        sb[kb][i] = 32 * kb + 8 * (i >> 2) + (i & 3) < rel ? t : kNegInf;
+                    }
+                kx = 1.f;  // already applied
+                lv = 0.f;
+            }
+            if (tail && bad_keys != 0) {  // rows that see a key whose V is no number
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++) {
+                    const uint32_t w = (uint32_t)(bad_keys >> (32 * kb)) >> (4 * lh);
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if ((w & (1u << (8 * (i >> 2) + (i & 3)))) && sb[kb][i] != kNegInf) sb[kb][i] = __builtin_nanf("");
+                }
+            }
+            float mx[2] = {sb[0][0], sb[1][0]};
+#pragma unroll
+            for (int i = 1; i < 16; i++) {
+                mx[0] = fmaxf(mx[0], sb[0][i]);
+                mx[1] = fmaxf(mx[1], sb[1][i]);
+            }
+            float mloc = __builtin_fmaf(fmaxf(mx[0], mx[1]), kx, lv);
+            const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mloc), __float_as_uint(mloc), false, false);
+            mloc = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+            if (__ballot(mloc > m_run + kSlack || (m_run == kNegInf && mloc > kNegInf))) {
+                const float mn = fmaxf(m_run, mloc);
+                const float alpha = __builtin_amdgcn_exp2f(m_run - (mn == kNegInf ? 0.f : mn));
+                m_run = mn;
+                l_run *= alpha;
+#pragma unroll
+                for (int db = 0; db < DB; db++) oacc[db] *= alpha;
+            }
+            const float off = lv - (m_run == kNegInf ? 0.f : m_run);
+            u32x4 pf[4];
+            float sum[2] = {0.f, 0.f};
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sb[kb][i], kx, off));
+                    const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sb[kb][i + 1], kx, off));
+                    sum[0] += e0;
+                    sum[1] += e1;
+                    pf[2 * kb + (i >> 3)][(i & 7) >> 1] = pack2<BF16>(e0, e1);
+                }
+            l_run = __builtin_fmaf(sum[0] + sum[1], inv_v, l_run);
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int db = 0; db < DB; db++)
+                    oacc[db] = mfma32<BF16>(*(lds_u32x4_ptr)(uintptr_t)(st + kK + (q * DB + db) * kOp), pf[q], oacc[db]);
+        };
+
+        if (tid == 0) bad_keys = 0;
+        __syncthreads();
+        float2 sc = {1.f, 1.f}, sc_next = sc;  // the scales of the block in LDS, and of the one in registers
+        int blk_next = b0 < bq ? table[b0] : 0;  // the table's entry for the block to load next: read a block ahead
+        auto fetch = [&](int j) {
+            const int blk = blk_next;
+            load(blk);
+            sc_next = reinterpret_cast<const float2*>(c.scales)[(int64_t)(blk >= 0 && blk < c.blocks ? blk : 0) * c.heads + h];
+            if (blk < 0 || blk >= c.blocks) sc_next.x = __builtin_nanf("");
+            if (j + 1 < bq) blk_next = table[j + 1];
+        };
+        auto advance = [&](int j, int buf) {  // block j into LDS, block j + 1 into registers
+            if (j < bq) {
+                stage(buf);
+                sc = sc_next;
+                if (j + 1 < bq) fetch(j + 1);
+            } else if (j < b1) {
+                stage_tail(buf);
+            }
+        };
+        if (b0 < bq) fetch(b0);
+        advance(b0, 0);
+        __syncthreads();
+        for (int j = b0; j < b1; j++) {
+            const int buf = (j - b0) & 1;
+            const bool tail = j >= nfull;
+            const float kx = tail ? p.c2 : sc.x * p.c2, lv = tail ? 0.f : __builtin_amdgcn_logf(sc.y);
+            advance(j + 1, buf ^ 1);
+            compute(j, buf, kx, lv, tail);
+            __syncthreads();
+        }
+
+        // ---- results ----
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
+        const float L = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+        if (row < rows) {
+            const int64_t at = s.t0 + (int64_t)tok;
+            if (nchunk == 1) {
+                const float inv = L == 0.f ? 0.f : 1.f / L;
+                uint16_t* dst = p.o + at * p.o_tok + hq * D + 4 * lh;
+#pragma unroll
+                for (int db = 0; db < DB; db++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++)
+                        *reinterpret_cast<u32x2*>(dst + 32 * db + 8 * q) =
+                            u32x2{pack2<BF16>(oacc[db][4 * q] * inv, oacc[db][4 * q + 1] * inv),
+                                  pack2<BF16>(oacc[db][4 * q + 2] * inv, oacc[db][4 * q + 3] * inv)};
+            } else {
+                const int64_t slot = (at * p.heads + hq) * p.chunks + ck;
+                float* dst = p.part + slot * D + 4 * lh;
+#pragma unroll
+                for (int db = 0; db < DB; db++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++)
+                        st4(dst + 32 * db + 8 * q,
+                            f32x4{oacc[db][4 * q], oacc[db][4 * q + 1], oacc[db][4 * q + 2], oacc[db][4 * q + 3]});
+                if (lh == 0)
+                    *reinterpret_cast<float2*>(p.part + (int64_t)p.max_tokens * p.heads * p.chunks * D + 2 * slot) =
+                        float2{m_run, L};
+            }
+        }
+    }
+}
+
 // ---- joining the chunks ----
 // One workgroup per row of o: its four waves take a quarter of the row's chunks each, eight loads in flight, and add up
 // in order.
@@ -470,7 +753,11 @@ hipError_t attend(const Kv8Attend& p, hipStream_t s) {
     const int64_t grid = (int64_t)p.c.requests * p.c.heads * p.tiles * p.chunks;
     if (grid <= 0 || grid > 0x7fffffff) return hipErrorInvalidValue;
     const dim3 g((unsigned)grid), b(64 * NW);
-    if (p.rows == 16 && p.once) hipLaunchKernelGGL((attend_few<CODE, BF16, D, 1, true>), g, b, 0, s, p);
+    if (p.kernel == kAttendMany) {
+        const int64_t eights = ((int64_t)p.c.requests * p.c.heads * p.chunks + 7) / 8;  // of (request, head, chunk)
+        hipLaunchKernelGGL((attend_many<CODE, BF16, D>), dim3((unsigned)(eights * 8 * p.tiles)), dim3(64 * MW), 0, s, p);
+    }
+    else if (p.rows == 16 && p.once) hipLaunchKernelGGL((attend_few<CODE, BF16, D, 1, true>), g, b, 0, s, p);
     else if (p.rows == 16) hipLaunchKernelGGL((attend_few<CODE, BF16, D, 1, false>), g, b, 0, s, p);
     else if (p.once) hipLaunchKernelGGL((attend_few<CODE, BF16, D, 2, true>), g, b, 0, s, p);
     else hipLaunchKernelGGL((attend_few<CODE, BF16, D, 2, false>), g, b, 0, s, p);
@@ -493,8 +780,8 @@ int64_t kv8_attend_plan(Kv8Attend& p, int head_dim, int max_new, int max_len, in
     const int64_t len = max_len > 0 && max_len < most ? max_len : most;
     const int64_t fresh = max_new > 0 && max_new < p.max_tokens ? max_new : p.max_tokens;
     const int64_t rows = fresh * p.group;
-    p.rows = rows <= 16 ? 16 : 32;
-    p.kernel = kAttendFew;
+    p.kernel = rows <= 32 ? kAttendFew : kAttendMany;
+    p.rows = p.kernel == kAttendMany ? MROWS : rows <= 16 ? 16 : 32;
     p.once = (int64_t)p.c.requests * len * p.c.heads * head_dim >= (int64_t)256 << 20;
     const int64_t tiles = (rows + p.rows - 1) / p.rows;
     p.tiles = (int32_t)(tiles < 1024 ? tiles : 1024);
@@ -504,12 +791,12 @@ int64_t kv8_attend_plan(Kv8Attend& p, int head_dim, int max_new, int max_len, in
     // (two requests of 262144 tokens, 8 heads of 128: 384 workgroups 134 us, 768 147, 1536 163; 32 requests of up to
     // 2048 tokens, 16 heads of 64: unsplit 18.3 us, in two with the join 20.2). Chunks are 8 to 128 blocks: shorter ones
     // are all start and merge, and a longer one would keep a single workgroup busy after the others.
-    const int64_t chunks_wanted = std::max<int64_t>(1, (int64_t)cus * few_waves(head_dim, p.rows / 16) / base);
+    const int64_t chunks_wanted = std::max<int64_t>(1, (int64_t)cus * (p.kernel == kAttendMany ? 2 : few_waves(head_dim, p.rows / 16)) / base);
     const int64_t chunk = std::min<int64_t>(128, std::max<int64_t>(8, (blocks + chunks_wanted - 1) / chunks_wanted));
     const int64_t chunks = (blocks + chunk - 1) / chunk;
     p.chunk = (int32_t)chunk;
     p.chunks = (int32_t)chunks;
-    if (base * chunks > INT32_MAX || (int64_t)p.max_tokens * p.heads > INT32_MAX) return -1;
+    if ((base + 8 * p.tiles) * chunks > INT32_MAX || (int64_t)p.max_tokens * p.heads > INT32_MAX) return -1;
     return chunks == 1 ? 0 : (int64_t)p.max_tokens * p.heads * chunks * (head_dim + 2) * 4;
 }
 
