@@ -401,7 +401,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(few_wav
 }
 
 // ---- many rows: tiles through LDS ----
-// One workgroup = (request, K/V head, 128 rows, chunk of the keys), four waves of 32 rows on v_mfma_f32_32x32x16. Each
+// One workgroup = (request, K/V head, 32 MW rows, chunk of the keys), MW waves of 32 rows on v_mfma_f32_32x32x16. Each
 // cache block is decoded once per workgroup, into LDS in the instructions' operand order, while the waves compute the
 // block before it; its codes are loaded a block earlier still. Lane l of a score block holds one row (l % 32) and keys
 // 8 (i / 4) + 4 (l / 32) + i % 4, i < 16: the order in which V's operand takes them, so the weights go from the scores'
@@ -416,17 +416,17 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-constexpr int MW = 4;          // waves
-constexpr int MROWS = 32 * MW;  // rows of a workgroup
 // The running max follows a block's only when it is passed by this much (exp2 units): weights up to 2^8 cost nothing,
 // and O is rescaled a few times per row instead of in every block.
 constexpr float kSlack = 8.f;
 
-template <int CODE, bool BF16, int D>
-__global__ __launch_bounds__(64 * MW) __attribute__((amdgpu_waves_per_eu(2, 2))) void attend_many(Kv8Attend p) {
+template <int CODE, bool BF16, int D, int MW>
+__global__ __launch_bounds__(64 * MW) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2))) void attend_many(Kv8Attend p) {
     constexpr int KS = D / 16;  // 16-dim steps of a score
     constexpr int DB = D / 32;  // 32-dim blocks of O
-    constexpr int U = D / 64;   // 16-byte pieces of K, and of V, per thread and block
+    constexpr int MROWS = 32 * MW;        // rows
+    constexpr int U = D / 16 / MW;        // 16-byte pieces of K, and of V, per thread and block
+    static_assert(U * MW * 16 == D, "every thread stages as much");
     // Operand blocks of 1 KB (lane l's 16 bytes at 16 l). K: (32 keys, 16-dim step); V: (16 keys, 32 dims).
     constexpr uint32_t kOp = 1024 + 128;  // 128 bytes apart: a staging wave's pieces of two steps lie on different banks
     constexpr uint32_t kK = 2 * KS * kOp, kStage = kK + 4 * DB * kOp;
@@ -470,7 +470,6 @@ __global__ __launch_bounds__(64 * MW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         const int tok = (int)(min(row, rows - 1) / G), hq = h * G + (int)(min(row, rows - 1) % G);
         const int kv_end = row < rows ? keys_to(s, tok) : 0;                                        // keys of the lane's row
         const int plain_end = wrow < rows ? keys_to(s, (int)(wrow / G)) : 0;                        // of all the wave's rows
-        const int wave_end = wrow < rows ? keys_to(s, (int)((min(rows, wrow + 32) - 1) / G)) : 0;  // of any
         u32x4 qf[KS];
 #pragma unroll
         for (int t = 0; t < KS; t++)
@@ -489,10 +488,10 @@ __global__ __launch_bounds__(64 * MW) __attribute__((amdgpu_waves_per_eu(2, 2)))
             const int64_t at = ((int64_t)(ok ? blk : 0) * c.heads + h) * kKvBlock * D;
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const int key = U == 1 ? 16 * wave + (lane & 15) : 16 * wave + 8 * u + (lane & 7);
-                const int step = U == 1 ? lane >> 4 : lane >> 3;
+                const int key = D == 64 ? 16 * (U * wave + u) + (lane & 15) : 8 * (U * wave + u) + (lane & 7);
+                const int step = D == 64 ? lane >> 4 : lane >> 3;
                 kc[u] = ld16(c.k + at + key * D + 16 * step);
-                const int dim = 16 * wave + 64 * u + (lane & 15);
+                const int dim = 16 * (U * wave + u) + (lane & 15);
                 vc[u] = ld16(c.v + at + dim * kKvBlock + 16 * (lane >> 4));
             }
         };
@@ -500,13 +499,13 @@ __global__ __launch_bounds__(64 * MW) __attribute__((amdgpu_waves_per_eu(2, 2)))
             const uint32_t st = lds0 + buf * kStage;
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const int key = U == 1 ? 16 * wave + (lane & 15) : 16 * wave + 8 * u + (lane & 7);
-                const int step = U == 1 ? lane >> 4 : lane >> 3;
+                const int key = D == 64 ? 16 * (U * wave + u) + (lane & 15) : 8 * (U * wave + u) + (lane & 7);
+                const int step = D == 64 ? lane >> 4 : lane >> 3;
                 const uint32_t a = st + ((key >> 5) * KS + step) * kOp + 16 * (key & 31);
                 *(lds_u32x4_ptr)(uintptr_t)a = decode8<CODE, BF16>(kc[u][0], kc[u][1]);
                 *(lds_u32x4_ptr)(uintptr_t)(a + 512) = decode8<CODE, BF16>(kc[u][2], kc[u][3]);
                 // V: words (c2, a2) of piece g are tokens 16 (2 c2 + a2) + 4 g .. + 3: four of the operand's eight slots
-                const int dim = 16 * wave + 64 * u + (lane & 15), g = lane >> 4;
+                const int dim = 16 * (U * wave + u) + (lane & 15), g = lane >> 4;
                 const uint32_t b = st + kK + (dim >> 5) * kOp + 16 * (32 * (g & 1) + (dim & 31)) + 8 * (g >> 1);
                 const u32x4 lo = decode8<CODE, BF16>(vc[u][0], vc[u][1]), hi = decode8<CODE, BF16>(vc[u][2], vc[u][3]);
                 *(lds_u32x2_ptr)(uintptr_t)(b) = u32x2{lo[0], lo[1]};
@@ -550,7 +549,6 @@ __global__ __launch_bounds__(64 * MW) __attribute__((amdgpu_waves_per_eu(2, 2)))
         // ---- one block ----
         auto compute = [&](int j, int buf, float kx, float lv, bool tail) {
             const int k0 = j * kKvBlock;
-            if (k0 >= wave_end) return;
             const float inv_v = __builtin_amdgcn_exp2f(-lv);
             const uint32_t st = lds0 + buf * kStage + 16 * lane;
             f32x16 sb[2] = {f32x16{}, f32x16{}};
@@ -590,7 +588,12 @@ __global__ __launch_bounds__(64 * MW) __attribute__((amdgpu_waves_per_eu(2, 2)))
             float mloc = __builtin_fmaf(fmaxf(mx[0], mx[1]), kx, lv);
             const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mloc), __float_as_uint(mloc), false, false);
             mloc = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-            if (__ballot(mloc > m_run + kSlack || (m_run == kNegInf && mloc > kNegInf))) {
+            // O follows the max rarely. The loop of at most one turn keeps its registers: around a branch the compiler holds O
+            // twice and copies it in every block, which costs what scaling it every time does.
+            int turns = __builtin_amdgcn_readfirstlane(__ballot(mloc > m_run + kSlack || (m_run == kNegInf && mloc > kNegInf)) != 0);
+            asm volatile("" : "+s"(turns));
+#pragma clang loop unroll(disable)
+            for (; turns > 0; turns--) {
                 const float mn = fmaxf(m_run, mloc);
                 const float alpha = __builtin_amdgcn_exp2f(m_run - (mn == kNegInf ? 0.f : mn));
                 m_run = mn;
@@ -684,13 +687,15 @@ __global__ __launch_bounds__(64 * MW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 }
 
 // ---- joining the chunks ----
-// One workgroup per row of o: its four waves take a quarter of the row's chunks each, eight loads in flight, and add up
-// in order.
-template <bool BF16, int D>
+// WPR waves per row of o, each taking its share of the row's chunks, eight loads in flight, and adding up in order: four
+// for the many chunks of few rows, one otherwise.
+template <bool BF16, int D, int WPR>
 __global__ __launch_bounds__(256) void attend_join(Kv8Attend p) {
     __shared__ float s_l[4], s_o[4][D];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int t = (int)(blockIdx.x / p.heads), hq = (int)(blockIdx.x % p.heads);
+    const int lane = threadIdx.x & 63, wave = WPR == 1 ? 0 : threadIdx.x >> 6;
+    const int64_t id = WPR == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    if (id >= (int64_t)p.max_tokens * p.heads) return;
+    const int t = (int)(id / p.heads), hq = (int)(id % p.heads);
     const Kv8& c = p.c;
     // The token's request: t itself where every request has one token, else the last r with cu[r] <= t.
     int r = min(t, c.requests - 1);
@@ -724,7 +729,7 @@ __global__ __launch_bounds__(256) void attend_join(Kv8Attend p) {
     float L = 0.f;
     constexpr int E = D / 64;
     float acc[E] = {};
-    const int k0 = n * wave / 4, k1 = n * (wave + 1) / 4;
+    const int k0 = n * wave / WPR, k1 = n * (wave + 1) / WPR;
 #pragma unroll 8
     for (int k = k0; k < k1; k++) {
         const float2 x = ml[k];
@@ -733,16 +738,20 @@ __global__ __launch_bounds__(256) void attend_join(Kv8Attend p) {
 #pragma unroll
         for (int e = 0; e < E; e++) acc[e] += f * part[(int64_t)k * D + E * lane + e];
     }
+    if constexpr (WPR > 1) {
 #pragma unroll
-    for (int e = 0; e < E; e++) s_o[wave][E * lane + e] = acc[e];
-    if (lane == 0) s_l[wave] = L;
-    __syncthreads();
-    if (wave) return;
-    L = ((s_l[0] + s_l[1]) + s_l[2]) + s_l[3];
+        for (int e = 0; e < E; e++) s_o[wave][E * lane + e] = acc[e];
+        if (lane == 0) s_l[wave] = L;
+        __syncthreads();
+        if (wave) return;
+        L = ((s_l[0] + s_l[1]) + s_l[2]) + s_l[3];
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            acc[e] = ((s_o[0][E * lane + e] + s_o[1][E * lane + e]) + s_o[2][E * lane + e]) + s_o[3][E * lane + e];
+    }
     const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
-    for (int e = 0; e < E; e++)
-        acc[e] = (((s_o[0][E * lane + e] + s_o[1][E * lane + e]) + s_o[2][E * lane + e]) + s_o[3][E * lane + e]) * inv;
+    for (int e = 0; e < E; e++) acc[e] *= inv;
     uint16_t* dst = p.o + (int64_t)t * p.o_tok + hq * D + E * lane;
     if constexpr (E == 1) *dst = (uint16_t)pack2<BF16>(acc[0], 0.f);
     else *reinterpret_cast<uint32_t*>(dst) = pack2<BF16>(acc[0], acc[1]);
@@ -755,7 +764,9 @@ hipError_t attend(const Kv8Attend& p, hipStream_t s) {
     const dim3 g((unsigned)grid), b(64 * NW);
     if (p.kernel == kAttendMany) {
         const int64_t eights = ((int64_t)p.c.requests * p.c.heads * p.chunks + 7) / 8;  // of (request, head, chunk)
-        hipLaunchKernelGGL((attend_many<CODE, BF16, D>), dim3((unsigned)(eights * 8 * p.tiles)), dim3(64 * MW), 0, s, p);
+        const dim3 gm((unsigned)(eights * 8 * p.tiles));
+        if (p.rows == 128) hipLaunchKernelGGL((attend_many<CODE, BF16, D, 4>), gm, dim3(256), 0, s, p);
+        else if constexpr (D == 128) hipLaunchKernelGGL((attend_many<CODE, BF16, D, 8>), gm, dim3(512), 0, s, p);
     }
     else if (p.rows == 16 && p.once) hipLaunchKernelGGL((attend_few<CODE, BF16, D, 1, true>), g, b, 0, s, p);
     else if (p.rows == 16) hipLaunchKernelGGL((attend_few<CODE, BF16, D, 1, false>), g, b, 0, s, p);
@@ -764,7 +775,10 @@ hipError_t attend(const Kv8Attend& p, hipStream_t s) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.chunks == 1) return e;
     const int64_t rows = (int64_t)p.max_tokens * p.heads;
-    hipLaunchKernelGGL((attend_join<BF16, D>), dim3((unsigned)rows), dim3(256), 0, s, p);
+    if (p.chunks <= 8)
+        hipLaunchKernelGGL((attend_join<BF16, D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, p);
+    else
+        hipLaunchKernelGGL((attend_join<BF16, D, 4>), dim3((unsigned)rows), dim3(256), 0, s, p);
     return hipGetLastError();
 }
 
@@ -781,7 +795,7 @@ int64_t kv8_attend_plan(Kv8Attend& p, int head_dim, int max_new, int max_len, in
     const int64_t fresh = max_new > 0 && max_new < p.max_tokens ? max_new : p.max_tokens;
     const int64_t rows = fresh * p.group;
     p.kernel = rows <= 32 ? kAttendFew : kAttendMany;
-    p.rows = p.kernel == kAttendMany ? MROWS : rows <= 16 ? 16 : 32;
+    p.rows = p.kernel == kAttendMany ? (head_dim == 128 && rows > 128 ? 256 : 128) : rows <= 16 ? 16 : 32;
     p.once = (int64_t)p.c.requests * len * p.c.heads * head_dim >= (int64_t)256 << 20;
     const int64_t tiles = (rows + p.rows - 1) / p.rows;
     p.tiles = (int32_t)(tiles < 1024 ? tiles : 1024);
@@ -791,7 +805,7 @@ int64_t kv8_attend_plan(Kv8Attend& p, int head_dim, int max_new, int max_len, in
     // (two requests of 262144 tokens, 8 heads of 128: 384 workgroups 134 us, 768 147, 1536 163; 32 requests of up to
     // 2048 tokens, 16 heads of 64: unsplit 18.3 us, in two with the join 20.2). Chunks are 8 to 128 blocks: shorter ones
     // are all start and merge, and a longer one would keep a single workgroup busy after the others.
-    const int64_t chunks_wanted = std::max<int64_t>(1, (int64_t)cus * (p.kernel == kAttendMany ? 2 : few_waves(head_dim, p.rows / 16)) / base);
+    const int64_t chunks_wanted = std::max<int64_t>(1, (int64_t)cus * (p.kernel == kAttendMany ? (p.rows == 256 ? 1 : 2) : few_waves(head_dim, p.rows / 16)) / base);
     const int64_t chunk = std::min<int64_t>(128, std::max<int64_t>(8, (blocks + chunks_wanted - 1) / chunks_wanted));
     const int64_t chunks = (blocks + chunk - 1) / chunk;
     p.chunk = (int32_t)chunk;
