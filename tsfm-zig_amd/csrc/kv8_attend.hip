@@ -401,7 +401,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(few_wav
 }
 
 // ---- many rows: tiles through LDS ----
-// One workgroup = (request, K/V head, 32 MW rows, chunk of the keys), MW waves of 32 rows on v_mfma_f32_32x32x16. Each
+// One workgroup = (request, K/V head, 128 rows, chunk of the keys), four waves of 32 rows on v_mfma_f32_32x32x16. Each
 // cache block is decoded once per workgroup, into LDS in the instructions' operand order, while the waves compute the
 // block before it; its codes are loaded a block earlier still. Lane l of a score block holds one row (l % 32) and keys
 // 8 (i / 4) + 4 (l / 32) + i % 4, i < 16: the order in which V's operand takes them, so the weights go from the scores'
@@ -416,15 +416,17 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
+constexpr int MW = 4;           // waves
+constexpr int MROWS = 32 * MW;  // rows of a workgroup (256 at 128 dims: 303 us where these take 273, 16 requests of 512
+                                // tokens and 4 heads a K/V head over 4096)
 // The running max follows a block's only when it is passed by this much (exp2 units): weights up to 2^8 cost nothing,
 // and O is rescaled a few times per row instead of in every block.
 constexpr float kSlack = 8.f;
 
-template <int CODE, bool BF16, int D, int MW>
+template <int CODE, bool BF16, int D>
 __global__ __launch_bounds__(64 * MW) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2))) void attend_many(Kv8Attend p) {
     constexpr int KS = D / 16;  // 16-dim steps of a score
     constexpr int DB = D / 32;  // 32-dim blocks of O
-    constexpr int MROWS = 32 * MW;        // rows
     constexpr int U = D / 16 / MW;        // 16-byte pieces of K, and of V, per thread and block
     static_assert(U * MW * 16 == D, "every thread stages as much");
     // Operand blocks of 1 KB (lane l's 16 bytes at 16 l). K: (32 keys, 16-dim step); V: (16 keys, 32 dims).
@@ -764,9 +766,7 @@ hipError_t attend(const Kv8Attend& p, hipStream_t s) {
     const dim3 g((unsigned)grid), b(64 * NW);
     if (p.kernel == kAttendMany) {
         const int64_t eights = ((int64_t)p.c.requests * p.c.heads * p.chunks + 7) / 8;  // of (request, head, chunk)
-        const dim3 gm((unsigned)(eights * 8 * p.tiles));
-        if (p.rows == 128) hipLaunchKernelGGL((attend_many<CODE, BF16, D, 4>), gm, dim3(256), 0, s, p);
-        else if constexpr (D == 128) hipLaunchKernelGGL((attend_many<CODE, BF16, D, 8>), gm, dim3(512), 0, s, p);
+        hipLaunchKernelGGL((attend_many<CODE, BF16, D>), dim3((unsigned)(eights * 8 * p.tiles)), dim3(64 * MW), 0, s, p);
     }
     else if (p.rows == 16 && p.once) hipLaunchKernelGGL((attend_few<CODE, BF16, D, 1, true>), g, b, 0, s, p);
     else if (p.rows == 16) hipLaunchKernelGGL((attend_few<CODE, BF16, D, 1, false>), g, b, 0, s, p);
@@ -794,8 +794,11 @@ int64_t kv8_attend_plan(Kv8Attend& p, int head_dim, int max_new, int max_len, in
     const int64_t len = max_len > 0 && max_len < most ? max_len : most;
     const int64_t fresh = max_new > 0 && max_new < p.max_tokens ? max_new : p.max_tokens;
     const int64_t rows = fresh * p.group;
-    p.kernel = rows <= 32 ? kAttendFew : kAttendMany;
-    p.rows = p.kernel == kAttendMany ? (head_dim == 128 && rows > 128 ? 256 : 128) : rows <= 16 ? 16 : 32;
+    // Whole tiles through LDS pay where there are many rows to share a block's decoding (us, tiles of 128 rows / of 32; four
+    // requests of up to 4096 tokens, 64 dims: 512 rows 69 / 42, 1024 84 / 66, 2048 95 / 103; 128 dims 57 / 44, 88 / 68,
+    // 119 / 122; 1200 rows over 20000 tokens 138 / 219; four prompts of up to 8192 rows over 8192 tokens 551 / 749).
+    p.kernel = rows <= 1024 ? kAttendFew : kAttendMany;
+    p.rows = p.kernel == kAttendMany ? MROWS : rows <= 16 ? 16 : 32;
     p.once = (int64_t)p.c.requests * len * p.c.heads * head_dim >= (int64_t)256 << 20;
     const int64_t tiles = (rows + p.rows - 1) / p.rows;
     p.tiles = (int32_t)(tiles < 1024 ? tiles : 1024);
@@ -805,7 +808,7 @@ int64_t kv8_attend_plan(Kv8Attend& p, int head_dim, int max_new, int max_len, in
     // (two requests of 262144 tokens, 8 heads of 128: 384 workgroups 134 us, 768 147, 1536 163; 32 requests of up to
     // 2048 tokens, 16 heads of 64: unsplit 18.3 us, in two with the join 20.2). Chunks are 8 to 128 blocks: shorter ones
     // are all start and merge, and a longer one would keep a single workgroup busy after the others.
-    const int64_t chunks_wanted = std::max<int64_t>(1, (int64_t)cus * (p.kernel == kAttendMany ? (p.rows == 256 ? 1 : 2) : few_waves(head_dim, p.rows / 16)) / base);
+    const int64_t chunks_wanted = std::max<int64_t>(1, (int64_t)cus * (p.kernel == kAttendMany ? 2 : few_waves(head_dim, p.rows / 16)) / base);
     const int64_t chunk = std::min<int64_t>(128, std::max<int64_t>(8, (blocks + chunks_wanted - 1) / chunks_wanted));
     const int64_t chunks = (blocks + chunk - 1) / chunk;
     p.chunk = (int32_t)chunk;
