@@ -199,21 +199,42 @@ __global__ __launch_bounds__(64 * FW) void gemm_few(F8Gemm p) {
     }
 }
 
+// Four consecutive results of a row at element `at`, the first `n` of them; ALIGNED: in one store.
+template <int OUT>
+__device__ __forceinline__ void store4(void* c, int64_t at, f32x4 v, int n, bool aligned) {
+    if (n >= 4 && aligned) {
+        if constexpr (OUT == 0) st4(static_cast<float*>(c) + at, v);
+        else
+            *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(c) + at) = u32x2{pack2<OUT == 1>(v[0], v[1]), pack2<OUT == 1>(v[2], v[3])};
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (i < n) store1<OUT>(c, at + i, v[i]);
+}
+
 // Tiles of TM x TN, WM x WN waves, a step of 128 values at a time. Both operands go from memory into LDS by DMA
 // (buffer loads whose descriptors end after the tile's rows: what is past m, n or k reads as 0), one step ahead,
 // one barrier per step. LDS rows are the step's 128 bytes with their 16-byte pieces XOR-swizzled by row.
-template <int OUT, int TM, int TN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void gemm_tiles(F8Gemm p) {
+// A wave's tile decides what LDS has to deliver: 64 x 64 needs 128 bytes a cycle where the matrix unit is kept busy, all
+// there is, 128 x 64 three quarters of it.
+template <int OUT, int TM, int TN, int WM, int WN, int OCC>
+__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void gemm_tiles(F8Gemm p) {
     constexpr int NWV = WM * WN, MT = TM / WM / 32, NT = TN / WN / 32;
     constexpr uint32_t kStage = (TM + TN) * KB;
+    static_assert(KB % (TN / WN) == 0, "a wave's columns share their scales");
     __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kStage];
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lr = lane & 31, lh = lane >> 5;
     const int mt_n = (p.m + TM - 1) / TM, nt_n = (p.n + TN - 1) / TN;
-    const int id = xcd_remap(blockIdx.x, gridDim.x);
-    const int m0 = (id % mt_n) * TM, n0 = (id / mt_n) * TN;
-    (void)nt_n;
+    // An XCD takes consecutive ids; they walk groups of 8 tiles of rows, so that the tiles in flight on it are about
+    // as many rows as columns and share their panels in its L2.
+    constexpr int GM = 8;
+    int id = xcd_remap(blockIdx.x, gridDim.x);
+    const int grp = id / (GM * nt_n), gm = min(GM, mt_n - grp * GM);
+    id -= grp * GM * nt_n;
+    const int m0 = (grp * GM + id % gm) * TM, n0 = id / gm * TN;
     const int wm = (wave % WM) * (TM / WM), wn = (wave / WM) * (TN / WN);
     const int kbs = (p.k + KB - 1) / KB;
     const int mrows = min(TM, p.m - m0), nrows = min(TN, p.n - n0);
@@ -223,26 +244,26 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tiles(F8Gemm p) {
     constexpr int AI = TM / 8 / NWV, BI = TN / 8 / NWV;
     constexpr uint32_t kOutside = 0x80000000u;  // past every descriptor (the host keeps a tile's rows below 2 GiB)
     const int srow = lane >> 3, spiece = (lane & 7) ^ (srow & 7);
+    const uint32_t a_off = (uint32_t)(wave * AI * 8 + srow) * (uint32_t)p.a_ld + 16u * spiece;
+    const uint32_t b_off = (uint32_t)(wave * BI * 8 + srow) * (uint32_t)p.b_ld + 16u * spiece;
     auto stage = [&](int kb, int buf) {
         const uint32_t st = lds0 + buf * kStage;
         const bool in = kb * KB + 16 * spiece < p.k;
 #pragma unroll
-        for (int i = 0; i < AI; i++) {
-            const int row = (wave * AI + i) * 8;
-            dma16(a_buf, st + row * KB, in ? (uint32_t)(row + srow) * (uint32_t)p.a_ld + 16u * spiece : kOutside,
+        for (int i = 0; i < AI; i++)
+            dma16(a_buf, st + (wave * AI + i) * 1024, in ? a_off + (uint32_t)(8 * i) * (uint32_t)p.a_ld : kOutside,
                   (uint32_t)kb * KB);
-        }
 #pragma unroll
-        for (int i = 0; i < BI; i++) {
-            const int row = (wave * BI + i) * 8;
-            dma16(b_buf, st + TM * KB + row * KB,
-                  in ? (uint32_t)(row + srow) * (uint32_t)p.b_ld + 16u * spiece : kOutside, (uint32_t)kb * KB);
-        }
+        for (int i = 0; i < BI; i++)
+            dma16(b_buf, st + TM * KB + (wave * BI + i) * 1024, in ? b_off + (uint32_t)(8 * i) * (uint32_t)p.b_ld : kOutside,
+                  (uint32_t)kb * KB);
     };
     typedef __attribute__((address_space(3))) u32x4* lds_ptr;
-    auto operand = [&](uint32_t base, int row, int s) {  // 32 bytes: pieces 4 s + 2 lh, + 1
-        const uint32_t r = base + row * KB, x = row & 7;
-        return pair(*(lds_ptr)(uintptr_t)(r + 16 * ((4 * s + 2 * lh) ^ x)), *(lds_ptr)(uintptr_t)(r + 16 * ((4 * s + 2 * lh + 1) ^ x)));
+    // 32 bytes of a row: pieces 4 s + 2 lh and the next, at their swizzled places (the row's low bits are the lane's).
+    const uint32_t sw0 = 16 * ((2 * lh) ^ (lr & 7)), sw1 = 16 * ((2 * lh + 1) ^ (lr & 7));
+    auto operand = [&](uint32_t row0, int s) {
+        const uint32_t r = row0 + lr * KB;
+        return pair(*(lds_ptr)(uintptr_t)(r + (sw0 ^ (64 * s))), *(lds_ptr)(uintptr_t)(r + (sw1 ^ (64 * s))));
     };
     f32x16 acc[MT][NT];
 #pragma unroll
@@ -254,33 +275,60 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tiles(F8Gemm p) {
     for (int i = 0; i < MT; i++) sa[i] = p.a_scales + (int64_t)min(m0 + wm + 32 * i + lr, p.m - 1) * p.a_scales_ld;
     const float* sb = p.b_scales + (int64_t)(min(n0 + wn, p.n - 1) / KB) * p.b_scales_ld;
 
+    float s[MT], s_next[MT];
+#pragma unroll
+    for (int i = 0; i < MT; i++) s_next[i] = sa[i][0] * sb[0];
     stage(0, 0);
     for (int kb = 0; kb < kbs; kb++) {
-        float s[MT];
 #pragma unroll
-        for (int i = 0; i < MT; i++) s[i] = sa[i][kb] * sb[kb];
+        for (int i = 0; i < MT; i++) s[i] = s_next[i];
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        if (kb + 1 < kbs) stage(kb + 1, (kb + 1) & 1);
-        const uint32_t st = lds0 + (kb & 1) * kStage;
-        Operand<OUT == 0> a[MT][2];
+        if (kb + 1 < kbs) {
+            stage(kb + 1, (kb + 1) & 1);
 #pragma unroll
-        for (int i = 0; i < MT; i++)
+            for (int i = 0; i < MT; i++) s_next[i] = sa[i][kb + 1] * sb[kb + 1];
+        }
+        const uint32_t st = lds0 + (kb & 1) * kStage, ra = st + wm * KB, rb = st + (TM + wn) * KB;
+        if constexpr (OUT != 0) {
+            Operand<false> a[MT][2];
 #pragma unroll
-            for (int h = 0; h < 2; h++) a[i][h].set(operand(st, wm + 32 * i + lr, h));
+            for (int i = 0; i < MT; i++)
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
-            Operand<OUT == 0> b[2];
+                for (int h = 0; h < 2; h++) a[i][h].set(operand(ra + 32 * i * KB, h));
 #pragma unroll
-            for (int h = 0; h < 2; h++) b[h].set(operand(st + TM * KB, wn + 32 * j + lr, h));
+            for (int j = 0; j < NT; j++) {
+                Operand<false> b[2];
 #pragma unroll
-            for (int i = 0; i < MT; i++) {
-                f32x16 x = mul(b[0], a[i][0], f32x16{});
-                x = mul(b[1], a[i][1], x);
+                for (int h = 0; h < 2; h++) b[h].set(operand(rb + 32 * j * KB, h));
 #pragma unroll
-                for (int r = 0; r < 16; r++) acc[i][j][r] = __builtin_fmaf(s[i], x[r], acc[i][j][r]);
+                for (int i = 0; i < MT; i++) {
+                    const f32x16 x = mul(b[1], a[i][1], mul(b[0], a[i][0], f32x16{}));
+#pragma unroll
+                    for (int r = 0; r < 16; r++) acc[i][j][r] = __builtin_fmaf(s[i], x[r], acc[i][j][r]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {  // half a step at a time: f16 operands are twice as large
+                Operand<true> b[NT];
+#pragma unroll
+                for (int j = 0; j < NT; j++) b[j].set(operand(rb + 32 * j * KB, h));
+#pragma unroll
+                for (int i = 0; i < MT; i++) {
+                    Operand<true> a;
+                    a.set(operand(ra + 32 * i * KB, h));
+#pragma unroll
+                    for (int j = 0; j < NT; j++) {
+                        const f32x16 x = mul(b[j], a, f32x16{});
+#pragma unroll
+                        for (int r = 0; r < 16; r++) acc[i][j][r] = __builtin_fmaf(s[i], x[r], acc[i][j][r]);
+                    }
+                }
             }
         }
     }
+    constexpr int kElem = OUT == 0 ? 4 : 2;
+    const bool aligned = p.c_ld % 4 == 0 && ((uintptr_t)p.c & (4 * kElem - 1)) == 0;
 #pragma unroll
     for (int i = 0; i < MT; i++) {
         const int m = m0 + wm + 32 * i + lr;
@@ -288,15 +336,24 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_tiles(F8Gemm p) {
 #pragma unroll
         for (int j = 0; j < NT; j++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int n = n0 + wn + 32 * j + 8 * (r >> 2) + 4 * lh + (r & 3);
-                if (n < p.n) store1<OUT>(p.c, m * p.c_ld + n, acc[i][j][r]);
+            for (int q = 0; q < 4; q++) {
+                const int n = n0 + wn + 32 * j + 8 * q + 4 * lh;
+                const f32x16& x = acc[i][j];
+                store4<OUT>(p.c, m * p.c_ld + n, f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]}, p.n - n, aligned);
             }
     }
 }
 
+template <int OUT, int TM, int TN, int WM, int WN, int OCC>
+hipError_t tiles(const F8Gemm& p, hipStream_t s) {
+    const int64_t grid = (((int64_t)p.m + TM - 1) / TM) * (((int64_t)p.n + TN - 1) / TN);
+    if (grid > 0x7fffffff) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((gemm_tiles<OUT, TM, TN, WM, WN, OCC>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, s, p);
+    return hipGetLastError();
+}
+
 template <int OUT>
-hipError_t gemm(const F8Gemm& p, int /*cus*/, hipStream_t s) {
+hipError_t gemm(const F8Gemm& p, int cus, hipStream_t s) {
     if (p.m <= 64) {
         const dim3 grid((unsigned)((p.n + 15) / 16)), block(64 * FW);
         if (p.m <= 16) hipLaunchKernelGGL((gemm_few<OUT, 1>), grid, block, 0, s, p);
@@ -304,10 +361,9 @@ hipError_t gemm(const F8Gemm& p, int /*cus*/, hipStream_t s) {
         else hipLaunchKernelGGL((gemm_few<OUT, 4>), grid, block, 0, s, p);
         return hipGetLastError();
     }
-    const int64_t grid = (((int64_t)p.m + 127) / 128) * ((p.n + 127) / 128);
-    if (grid > 0x7fffffff) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((gemm_tiles<OUT, 128, 128, 2, 2>), dim3((unsigned)grid), dim3(256), 0, s, p);
-    return hipGetLastError();
+    const int64_t big = (((int64_t)p.m + 255) / 256) * (((int64_t)p.n + 255) / 256);
+    if (big >= cus) return tiles<OUT, 256, 256, 2, 4, 2>(p, s);
+    return tiles<OUT, 128, 128, 2, 2, 2>(p, s);
 }
 
 template <int DTYPE>
