@@ -224,6 +224,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(OC
     constexpr uint32_t kStage = (TM + TN) * KB;
     static_assert(KB % (TN / WN) == 0, "a wave's columns share their scales");
     __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kStage];
+    __shared__ float scales[2][4][TM];
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lr = lane & 31, lh = lane >> 5;
@@ -270,24 +271,45 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(OC
     for (int i = 0; i < MT; i++)
 #pragma unroll
         for (int j = 0; j < NT; j++) acc[i][j] = f32x16{};
-    const float* sa[MT];
+    // a's scales: each of the first TM threads keeps its row's, four steps at a time (one 16-byte load, and as many
+    // cache lines as rows; a load per step and wave asked for sixteen times as many), and puts them into LDS by step.
+    const int srow_m = min(m0 + (int)threadIdx.x, p.m - 1);
+    const float* const sa = p.a_scales + (int64_t)srow_m * p.a_scales_ld;
+    const bool scaler = threadIdx.x < TM;
+    typedef f32x4 f32x4_any __attribute__((aligned(4)));
+    auto load_scales = [&](int kb) {
+        f32x4 v = {0, 0, 0, 0};
+        if (kb + 4 <= kbs) v = *reinterpret_cast<const f32x4_any*>(sa + kb);
+        else
 #pragma unroll
-    for (int i = 0; i < MT; i++) sa[i] = p.a_scales + (int64_t)min(m0 + wm + 32 * i + lr, p.m - 1) * p.a_scales_ld;
+            for (int i = 0; i < 3; i++)
+                if (kb + i < kbs) v[i] = sa[kb + i];
+        return v;
+    };
+    auto put_scales = [&](f32x4 v, int buf) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) scales[buf][i][threadIdx.x] = v[i];
+    };
     const float* sb = p.b_scales + (int64_t)(min(n0 + wn, p.n - 1) / KB) * p.b_scales_ld;
 
-    float s[MT], s_next[MT];
-#pragma unroll
-    for (int i = 0; i < MT; i++) s_next[i] = sa[i][0] * sb[0];
+    f32x4 ahead = {0, 0, 0, 0};
+    if (scaler) put_scales(load_scales(0), 0);
+    float sb_next = sb[0];
     stage(0, 0);
     for (int kb = 0; kb < kbs; kb++) {
-#pragma unroll
-        for (int i = 0; i < MT; i++) s[i] = s_next[i];
-        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        const float sbk = sb_next;
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (kb + 1 < kbs) {
             stage(kb + 1, (kb + 1) & 1);
-#pragma unroll
-            for (int i = 0; i < MT; i++) s_next[i] = sa[i][kb + 1] * sb[kb + 1];
+            sb_next = sb[kb + 1];
         }
+        if (scaler) {  // whole waves
+            if ((kb & 3) == 0 && kb + 4 < kbs) ahead = load_scales(kb + 4);
+            if ((kb & 3) == 3) put_scales(ahead, ((kb >> 2) + 1) & 1);
+        }
+        float s[MT];
+#pragma unroll
+        for (int i = 0; i < MT; i++) s[i] = scales[(kb >> 2) & 1][kb & 3][wm + 32 * i + lr] * sbk;
         const uint32_t st = lds0 + (kb & 1) * kStage, ra = st + wm * KB, rb = st + (TM + wn) * KB;
         if constexpr (OUT != 0) {
             Operand<false> a[MT][2];
