@@ -215,7 +215,7 @@ __device__ __forceinline__ void store4(void* c, int64_t at, f32x4 v, int n, bool
 
 // Tiles of TM x TN, WM x WN waves, a step of 128 values at a time. Both operands go from memory into LDS by DMA
 // (buffer loads whose descriptors end after the tile's rows: what is past m, n or k reads as 0), one step ahead,
-// one barrier per step. LDS rows are the step's 128 bytes with their 16-byte pieces XOR-swizzled by row.
+// one barrier per step. LDS rows are the step's 128 bytes with their 16-byte pieces XOR-swizzled.
 // A wave's tile decides what LDS has to deliver: 64 x 64 needs 128 bytes a cycle where the matrix unit is kept busy, all
 // there is, 128 x 64 three quarters of it.
 template <int OUT, int TM, int TN, int WM, int WN, int OCC>
@@ -224,7 +224,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(OC
     constexpr uint32_t kStage = (TM + TN) * KB;
     static_assert(KB % (TN / WN) == 0, "a wave's columns share their scales");
     __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kStage];
-    __shared__ float scales[2][4][TM];
+    __shared__ float scales[8][TN / KB][TM];
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lr = lane & 31, lh = lane >> 5;
@@ -244,24 +244,30 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(OC
     // One DMA instruction of a wave fills 1 KB: 8 rows, lane l piece l % 8 of row l / 8.
     constexpr int AI = TM / 8 / NWV, BI = TN / 8 / NWV;
     constexpr uint32_t kOutside = 0x80000000u;  // past every descriptor (the host keeps a tile's rows below 2 GiB)
-    const int srow = lane >> 3, spiece = (lane & 7) ^ (srow & 7);
-    const uint32_t a_off = (uint32_t)(wave * AI * 8 + srow) * (uint32_t)p.a_ld + 16u * spiece;
-    const uint32_t b_off = (uint32_t)(wave * BI * 8 + srow) * (uint32_t)p.b_ld + 16u * spiece;
+    // Pieces are swizzled by half the row: 16 lanes, which LDS serves together, read two rows a bank half and eight
+    // places in each. (By the row itself: every read two deep on its banks.)
+    static_assert(AI % 2 == 0 && BI % 2 == 0, "the swizzle's upper bit goes by the instruction's parity");
+    const int srow = lane >> 3, spiece = (lane & 7) ^ (srow >> 1);
+    const uint32_t a_off = (uint32_t)(wave * AI * 8 + srow) * (uint32_t)p.a_ld;
+    const uint32_t b_off = (uint32_t)(wave * BI * 8 + srow) * (uint32_t)p.b_ld;
     auto stage = [&](int kb, int buf) {
         const uint32_t st = lds0 + buf * kStage;
-        const bool in = kb * KB + 16 * spiece < p.k;
 #pragma unroll
-        for (int i = 0; i < AI; i++)
-            dma16(a_buf, st + (wave * AI + i) * 1024, in ? a_off + (uint32_t)(8 * i) * (uint32_t)p.a_ld : kOutside,
-                  (uint32_t)kb * KB);
+        for (int i = 0; i < AI; i++) {
+            const uint32_t at = 16u * (spiece ^ (4 * (i & 1)));
+            dma16(a_buf, st + (wave * AI + i) * 1024,
+                  kb * KB + (int)at < p.k ? a_off + (uint32_t)(8 * i) * (uint32_t)p.a_ld + at : kOutside, (uint32_t)kb * KB);
+        }
 #pragma unroll
-        for (int i = 0; i < BI; i++)
-            dma16(b_buf, st + TM * KB + (wave * BI + i) * 1024, in ? b_off + (uint32_t)(8 * i) * (uint32_t)p.b_ld : kOutside,
-                  (uint32_t)kb * KB);
+        for (int i = 0; i < BI; i++) {
+            const uint32_t at = 16u * (spiece ^ (4 * (i & 1)));
+            dma16(b_buf, st + TM * KB + (wave * BI + i) * 1024,
+                  kb * KB + (int)at < p.k ? b_off + (uint32_t)(8 * i) * (uint32_t)p.b_ld + at : kOutside, (uint32_t)kb * KB);
+        }
     };
     typedef __attribute__((address_space(3))) u32x4* lds_ptr;
     // 32 bytes of a row: pieces 4 s + 2 lh and the next, at their swizzled places (the row's low bits are the lane's).
-    const uint32_t sw0 = 16 * ((2 * lh) ^ (lr & 7)), sw1 = 16 * ((2 * lh + 1) ^ (lr & 7));
+    const uint32_t sw0 = 16 * ((2 * lh) ^ ((lr >> 1) & 7)), sw1 = 16 * ((2 * lh + 1) ^ ((lr >> 1) & 7));
     auto operand = [&](uint32_t row0, int s) {
         const uint32_t r = row0 + lr * KB;
         return pair(*(lds_ptr)(uintptr_t)(r + (sw0 ^ (64 * s))), *(lds_ptr)(uintptr_t)(r + (sw1 ^ (64 * s))));
@@ -271,63 +277,63 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(OC
     for (int i = 0; i < MT; i++)
 #pragma unroll
         for (int j = 0; j < NT; j++) acc[i][j] = f32x16{};
-    // a's scales: each of the first TM threads keeps its row's, four steps at a time (one 16-byte load, and as many
-    // cache lines as rows; a load per step and wave asked for sixteen times as many), and puts them into LDS by step.
-    const int srow_m = min(m0 + (int)threadIdx.x, p.m - 1);
-    const float* const sa = p.a_scales + (int64_t)srow_m * p.a_scales_ld;
-    const bool scaler = threadIdx.x < TM;
+    // The scales' products, by step, row and 128 columns, in LDS: a thread keeps one row and column group, four steps at a
+    // time (16-byte loads; a load per step, wave and row asked for sixteen times as many cache lines). Steps k and k + 8
+    // share a place. Loads and writes come before the step's copies: the wait for them would wait for those too.
+    const int sgrp = threadIdx.x / TM;
+    const bool scaler = sgrp < TN / KB;  // whole waves
+    const float* const sa = p.a_scales + (int64_t)min(m0 + (int)(threadIdx.x % TM), p.m - 1) * p.a_scales_ld;
+    const float* const sb = p.b_scales + (int64_t)min(n0 / KB + min(sgrp, TN / KB - 1), (p.n - 1) / KB) * p.b_scales_ld;
     typedef f32x4 f32x4_any __attribute__((aligned(4)));
-    auto load_scales = [&](int kb) {
-        f32x4 v = {0, 0, 0, 0};
-        if (kb + 4 <= kbs) v = *reinterpret_cast<const f32x4_any*>(sa + kb);
-        else
-#pragma unroll
-            for (int i = 0; i < 3; i++)
-                if (kb + i < kbs) v[i] = sa[kb + i];
-        return v;
-    };
-    auto put_scales = [&](f32x4 v, int buf) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) scales[buf][i][threadIdx.x] = v[i];
-    };
-    const float* sb = p.b_scales + (int64_t)(min(n0 + wn, p.n - 1) / KB) * p.b_scales_ld;
-
-    f32x4 ahead = {0, 0, 0, 0};
-    if (scaler) put_scales(load_scales(0), 0);
-    float sb_next = sb[0];
+    auto put = [&](int k, float v) { scales[k & 7][sgrp][threadIdx.x % TM] = v; };
+    f32x4 va = {0, 0, 0, 0}, vb = va;
+    if (scaler)
+        for (int k = 0; k < min(4, kbs); k++) put(k, sa[k] * sb[k]);
     stage(0, 0);
     for (int kb = 0; kb < kbs; kb++) {
-        const float sbk = sb_next;
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (kb + 1 < kbs) {
-            stage(kb + 1, (kb + 1) & 1);
-            sb_next = sb[kb + 1];
+        const int ahead = min((kb & ~3) + 4, kbs - 4);  // steps whose scales are fetched now; at the end some again
+        if (scaler && (kb | 3) + 1 < kbs) {
+            if ((kb & 3) == 0) {
+                va = *reinterpret_cast<const f32x4_any*>(sa + ahead);
+                vb = *reinterpret_cast<const f32x4_any*>(sb + ahead);
+            }
+            if ((kb & 3) == 3)
+#pragma unroll
+                for (int i = 0; i < 4; i++) put(ahead + i, va[i] * vb[i]);
         }
-        if (scaler) {  // whole waves
-            if ((kb & 3) == 0 && kb + 4 < kbs) ahead = load_scales(kb + 4);
-            if ((kb & 3) == 3) put_scales(ahead, ((kb >> 2) + 1) & 1);
-        }
+        if (kb + 1 < kbs) stage(kb + 1, (kb + 1) & 1);
         float s[MT];
 #pragma unroll
-        for (int i = 0; i < MT; i++) s[i] = scales[(kb >> 2) & 1][kb & 3][wm + 32 * i + lr] * sbk;
+        for (int i = 0; i < MT; i++) s[i] = scales[kb & 7][wn / KB][wm + 32 * i + lr];
         const uint32_t st = lds0 + (kb & 1) * kStage, ra = st + wm * KB, rb = st + (TM + wn) * KB;
         if constexpr (OUT != 0) {
-            Operand<false> a[MT][2];
+            // Tile by tile, the products of one issued before the multiply-adds of the one before: the vector unit works on
+            // those while the matrix unit is at the next. a's operands are read a tile row ahead.
+            Operand<false> b[NT][2], a[2][2];
 #pragma unroll
-            for (int i = 0; i < MT; i++)
+            for (int h = 0; h < 2; h++) {
+                a[0][h].set(operand(ra, h));
 #pragma unroll
-                for (int h = 0; h < 2; h++) a[i][h].set(operand(ra + 32 * i * KB, h));
+                for (int j = 0; j < NT; j++) b[j][h].set(operand(rb + 32 * j * KB, h));
+            }
+            f32x16 x[2];
 #pragma unroll
-            for (int j = 0; j < NT; j++) {
-                Operand<false> b[2];
+            for (int t = 0; t <= MT * NT; t++) {
+                const int i = t / NT, j = t % NT;
+                if (t < MT * NT) {
+                    if (j == 0 && i + 1 < MT)
 #pragma unroll
-                for (int h = 0; h < 2; h++) b[h].set(operand(rb + 32 * j * KB, h));
-#pragma unroll
-                for (int i = 0; i < MT; i++) {
-                    const f32x16 x = mul(b[1], a[i][1], mul(b[0], a[i][0], f32x16{}));
-#pragma unroll
-                    for (int r = 0; r < 16; r++) acc[i][j][r] = __builtin_fmaf(s[i], x[r], acc[i][j][r]);
+                        for (int h = 0; h < 2; h++) a[(i + 1) & 1][h].set(operand(ra + 32 * (i + 1) * KB, h));
+                    x[t & 1] = mul(b[j][1], a[i & 1][1], mul(b[j][0], a[i & 1][0], f32x16{}));
                 }
+                if (t > 0) {
+                    const int u = t - 1;
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        acc[u / NT][u % NT][r] = __builtin_fmaf(s[u / NT], x[u & 1][r], acc[u / NT][u % NT][r]);
+                }
+                __builtin_amdgcn_sched_barrier(0x100);  // in this order but for the reads of LDS
             }
         } else {
 #pragma unroll
