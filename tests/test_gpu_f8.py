@@ -155,6 +155,35 @@ def test_product_matches_float64(ta, gpu_ready, name, m, n, k):
     assert (err <= bound).all(), float((err / bound).max())
 
 
+# Few rows by 16, 32 and 64 columns a workgroup, tiles of 128 and of 256; reductions of 1 to 10 blocks.
+WIDE = [(9, 4200, 144), (16, 8300, 272), (1, 16, 1280), (30, 4100, 256), (31, 8209, 144), (60, 4000, 1296),
+        (130, 2100, 1152), (300, 2000, 1040), (20, 20000, 144), (1000, 2999, 656), (1100, 2900, 512), (2600, 1000, 896),
+        (3500, 4200, 656), (3700, 4099, 128), (4000, 4096, 1040)]
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("m,n,k", WIDE)
+def test_product_of_every_tile(ta, gpu_ready, name, m, n, k):
+    """Each of the kernels, with rows of the result that start at 16 bytes and rows that do not: the same bits, within
+    the bound, nothing written beside them."""
+    torch = _t()
+    rng = np.random.default_rng(m + n + k)
+    a, ad, sa, sad, b, bd, sb, sbd = _operands(rng, m, n, k, pad=16)
+    odd = torch.full((m + 1, n + 3 - n % 2), -7.0, dtype=_dtype(name), device="cuda")
+    even = torch.full((m + 1, (n + 31) // 16 * 16), -7.0, dtype=_dtype(name), device="cuda")
+    for wide in (odd, even):
+        assert ta.f8_gemm_nt(ad, sad, bd, sbd, wide[:m, :n]) == ta.OK, ta.last_error()
+        assert (wide[m:] == -7).all() and (wide[:, n:] == -7).all()
+    assert torch.equal(odd[:m, :n], even[:m, :n])
+    c, S, M = _product_ref(a, sa, b, sb)
+    got = even[:m, :n].double()
+    bound = _bound(c, S, M, name, sa.shape[1])
+    ok = (got - c).abs() <= bound
+    if name == "f16":  # a result that rounds past the largest value is an infinity
+        ok |= got.isinf() & (c.abs() + bound >= torch.finfo(torch.float16).max)
+    assert ok.all(), ((got - c).abs() / bound).max()
+
+
 @pytest.mark.parametrize("m", [3, 70, 300])
 @pytest.mark.parametrize("name", ["f32", "bf16"])
 def test_a_nan_stays_in_its_row_and_column(ta, gpu_ready, m, name):

@@ -152,53 +152,6 @@ __device__ __forceinline__ void store1(void* c, int64_t at, float v) {
     else static_cast<uint16_t*>(c)[at] = (uint16_t)pack2<OUT == 1>(v, 0.f);
 }
 
-// Few rows of a (16 MT): one workgroup per 16 rows of b, its waves sharing the reduction by blocks of 128 and
-// adding up through LDS in order. b is read once, straight into the operands: bound by its bytes, or by latency.
-constexpr int FW = 8;
-template <int OUT, int MT>
-__global__ __launch_bounds__(64 * FW) void gemm_few(F8Gemm p) {
-    __shared__ float part[FW][MT][64][4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int ql = lane & 15, g = lane >> 4;
-    const int n0 = blockIdx.x * 16, kbs = (p.k + KB - 1) / KB;
-    const int64_t brow = (int64_t)min(n0 + ql, p.n - 1) * p.b_ld;
-    f32x4 acc[MT];
-#pragma unroll
-    for (int t = 0; t < MT; t++) acc[t] = f32x4{0, 0, 0, 0};
-    auto load = [&](const uint8_t* row, int kb) {  // the lane's 32 bytes of block kb; 0 past k
-        const int k0 = kb * KB + 32 * g;
-        const u32x4 z = {0, 0, 0, 0};
-        return pair(k0 < p.k ? ld16(row + k0) : z, k0 + 16 < p.k ? ld16(row + k0 + 16) : z);
-    };
-    for (int kb = wave; kb < kbs; kb += FW) {
-        Operand<OUT == 0> b, a;
-        b.set(load(p.b + brow, kb));
-        const float sb = p.b_scales[(int64_t)(n0 / KB) * p.b_scales_ld + kb];
-#pragma unroll
-        for (int t = 0; t < MT; t++) {
-            const int64_t m = min(16 * t + ql, p.m - 1);
-            a.set(load(p.a + m * p.a_ld, kb));
-            const float s = sb * p.a_scales[m * p.a_scales_ld + kb];
-            const f32x4 x = mul(b, a, f32x4{0, 0, 0, 0});
-#pragma unroll
-            for (int i = 0; i < 4; i++) acc[t][i] = __builtin_fmaf(s, x[i], acc[t][i]);
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < MT; t++) st4(part[wave][t][lane], acc[t]);
-    __syncthreads();
-    for (int t = wave; t < MT; t += FW) {
-        f32x4 sum = {0, 0, 0, 0};
-#pragma unroll
-        for (int w = 0; w < FW; w++) sum += ld4(part[w][t][lane]);
-        const int m = 16 * t + ql;  // the lane's results: rows n0 + 4 g + i of b
-        if (m < p.m)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (n0 + 4 * g + i < p.n) store1<OUT>(p.c, m * p.c_ld + n0 + 4 * g + i, sum[i]);
-    }
-}
-
 // Four consecutive results of a row at element `at`, the first `n` of them; ALIGNED: in one store.
 template <int OUT>
 __device__ __forceinline__ void store4(void* c, int64_t at, f32x4 v, int n, bool aligned) {
@@ -211,6 +164,90 @@ __device__ __forceinline__ void store4(void* c, int64_t at, f32x4 v, int n, bool
 #pragma unroll
     for (int i = 0; i < 4; i++)
         if (i < n) store1<OUT>(c, at + i, v[i]);
+}
+
+// 16 MT rows of a by 16 NT rows of b a workgroup, whose eight waves share the reduction by blocks of 128 and add up
+// through LDS in order. Operands come straight from memory into registers, a block ahead: a load covers 16 rows of 64
+// consecutive bytes. For few rows, bound by the bytes of b, and for products whose tiles would not fill the CUs, bound by
+// latency: that of k / 1024 loads here.
+constexpr int FW = 8;
+template <int OUT, int MT, int NT>
+__global__ __launch_bounds__(64 * FW) void gemm_few(F8Gemm p) {
+    __shared__ __attribute__((aligned(16))) float part[FW][MT * NT][64][4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ql = lane & 15, g = lane >> 4;
+    const int mt_n = (p.m + 16 * MT - 1) / (16 * MT), kbs = (p.k + KB - 1) / KB;
+    const int id = xcd_remap(blockIdx.x, gridDim.x);
+    const int m0 = id % mt_n * 16 * MT, n0 = id / mt_n * 16 * NT;
+    static_assert(KB % (16 * NT) == 0, "b's rows share their scales");
+    const uint8_t *ra[MT], *rb[NT];
+    const float* sa[MT];
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+        const int64_t m = min(m0 + 16 * i + ql, p.m - 1);
+        ra[i] = p.a + m * p.a_ld;
+        sa[i] = p.a_scales + m * p.a_scales_ld;
+    }
+#pragma unroll
+    for (int j = 0; j < NT; j++) rb[j] = p.b + (int64_t)min(n0 + 16 * j + ql, p.n - 1) * p.b_ld;
+    const float* const sb = p.b_scales + (int64_t)(n0 / KB) * p.b_scales_ld;
+    i32x8 a[MT], b[NT];
+    float s[MT];
+    auto load = [&](int kb) {  // pieces g and 4 + g of the block's 128 bytes; 0 past k
+        const int k0 = kb * KB + 16 * g;
+        const bool lo = k0 < p.k, hi = k0 + 64 < p.k;
+        const u32x4 z = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < NT; j++) b[j] = pair(lo ? ld16(rb[j] + k0) : z, hi ? ld16(rb[j] + k0 + 64) : z);
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            a[i] = pair(lo ? ld16(ra[i] + k0) : z, hi ? ld16(ra[i] + k0 + 64) : z);
+            s[i] = sa[i][kb] * sb[kb];
+        }
+    };
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) acc[i][j] = f32x4{0, 0, 0, 0};
+    if (wave < kbs) load(wave);
+    for (int kb = wave; kb < kbs; kb += FW) {
+        Operand<OUT == 0> ob[NT], oa;
+        i32x8 ac[MT];
+        float sc[MT];
+#pragma unroll
+        for (int j = 0; j < NT; j++) ob[j].set(b[j]);
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            ac[i] = a[i];
+            sc[i] = s[i];
+        }
+        if (kb + FW < kbs) load(kb + FW);
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            oa.set(ac[i]);
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                const f32x4 x = mul(ob[j], oa, f32x4{0, 0, 0, 0});
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[i][j][r] = __builtin_fmaf(sc[i], x[r], acc[i][j][r]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) st4(part[wave][i * NT + j][lane], acc[i][j]);
+    __syncthreads();
+    constexpr int kElem = OUT == 0 ? 4 : 2;
+    const bool aligned = p.c_ld % 4 == 0 && ((uintptr_t)p.c & (4 * kElem - 1)) == 0;
+    for (int t = wave; t < MT * NT; t += FW) {
+        f32x4 sum = ld4(part[0][t][lane]);
+#pragma unroll
+        for (int w = 1; w < FW; w++) sum += ld4(part[w][t][lane]);
+        const int m = m0 + 16 * (t / NT) + ql, n = n0 + 16 * (t % NT) + 4 * g;  // the lane's results: n .. n + 3
+        if (m < p.m) store4<OUT>(p.c, m * p.c_ld + n, sum, p.n - n, aligned);
+    }
 }
 
 // Tiles of TM x TN, WM x WN waves, a step of 128 values at a time. Both operands go from memory into LDS by DMA
@@ -355,19 +392,48 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(OC
             }
         }
     }
-    constexpr int kElem = OUT == 0 ? 4 : 2;
+    // Results: 32 rows of the wave's columns at a time through its part of LDS, so that a store writes whole lines (8 bytes
+    // a row and lane straight from the registers: 80 us of 617 at 16384 x 8192 x 4096).
+    constexpr int kElem = OUT == 0 ? 4 : 2, kRow = TN / WN * kElem, kPad = kRow + 16;  // bytes of a row, and in LDS
+    constexpr int LR = kRow / 16, RL = 64 / LR;                                         // lanes per row, rows per store
+    static_assert(32 * kPad * NWV <= (int)sizeof(smem), "a part of LDS for every wave");
+    const bool whole = p.c_ld * kElem % 16 == 0 && ((uintptr_t)p.c & 15) == 0 && n0 + wn + TN / WN <= p.n;
     const bool aligned = p.c_ld % 4 == 0 && ((uintptr_t)p.c & (4 * kElem - 1)) == 0;
+    asm volatile("s_barrier" ::: "memory");  // every wave has its last operands
+    const uint32_t part = lds0 + wave * 32 * kPad;
+    typedef __attribute__((address_space(3))) u32x2* lds8_ptr;
 #pragma unroll
     for (int i = 0; i < MT; i++) {
-        const int m = m0 + wm + 32 * i + lr;
-        if (m >= p.m) continue;
+        const int mrow = m0 + wm + 32 * i;
+        if (whole) {
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const f32x16& x = acc[i][j];
+                    const uint32_t at = part + lr * kPad + (32 * j + 8 * q + 4 * lh) * kElem;
+                    if constexpr (OUT == 0)
+                        *(lds_ptr)(uintptr_t)at = __builtin_bit_cast(u32x4, f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]});
+                    else
+                        *(lds8_ptr)(uintptr_t)at = u32x2{pack2<OUT == 1>(x[4 * q], x[4 * q + 1]), pack2<OUT == 1>(x[4 * q + 2], x[4 * q + 3])};
+                }
+#pragma unroll
+            for (int t = 0; t < 32; t += RL) {
+                const int row = t + lane / LR;
+                const u32x4 v = *(lds_ptr)(uintptr_t)(part + row * kPad + 16 * (lane % LR));
+                if (mrow + row < p.m)
+                    *reinterpret_cast<u32x4*>(static_cast<char*>(p.c) + ((mrow + row) * p.c_ld + n0 + wn) * kElem + 16 * (lane % LR)) = v;
+            }
+            continue;
+        }
+        if (mrow + lr >= p.m) continue;
 #pragma unroll
         for (int j = 0; j < NT; j++)
 #pragma unroll
             for (int q = 0; q < 4; q++) {
                 const int n = n0 + wn + 32 * j + 8 * q + 4 * lh;
                 const f32x16& x = acc[i][j];
-                store4<OUT>(p.c, m * p.c_ld + n, f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]}, p.n - n, aligned);
+                store4<OUT>(p.c, (mrow + lr) * p.c_ld + n, f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]}, p.n - n, aligned);
             }
     }
 }
@@ -380,17 +446,44 @@ hipError_t tiles(const F8Gemm& p, hipStream_t s) {
     return hipGetLastError();
 }
 
+template <int OUT, int MT, int NT>
+hipError_t few(const F8Gemm& p, hipStream_t s) {
+    const int64_t grid = (((int64_t)p.m + 16 * MT - 1) / (16 * MT)) * (((int64_t)p.n + 16 * NT - 1) / (16 * NT));
+    if (grid > 0x7fffffff) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((gemm_few<OUT, MT, NT>), dim3((unsigned)grid), dim3(64 * FW), 0, s, p);
+    return hipGetLastError();
+}
+
+// gemm_few with the narrowest columns whose workgroups all run at once, one a CU; false if no width does.
+template <int OUT, int MT>
+bool few(const F8Gemm& p, int cus, hipStream_t s, hipError_t& err) {
+    const int64_t mt = ((int64_t)p.m + 16 * MT - 1) / (16 * MT), n16 = ((int64_t)p.n + 15) / 16;
+    if (mt * n16 <= cus) err = few<OUT, MT, 1>(p, s);
+    else if (mt * ((n16 + 1) / 2) <= cus) err = few<OUT, MT, 2>(p, s);
+    else if (MT == 1 || mt * ((n16 + 3) / 4) <= cus) err = few<OUT, MT, 4>(p, s);
+    else return false;
+    return true;
+}
+
+// Which kernel, measured on 256 CUs, us for m x n x k, bf16 results.
+// gemm_few where its workgroups run at once: its waves split k, so that the chain of loads is an eighth as long as that
+// of tiles: 64 x 2048 x 4096 14.7 against 25.0, 400 x 512 x 2048 8.5 against 14.3, 800 x 1024 x 4096 22.0 against 25.6.
+// Its columns, 16 / 32 / 64: 16 x 4096 x 1024 3.3 / 3.8 / 4.7; 16 x 8192 x 2048 6.7 / 5.4 / 7.3;
+// 16 x 16384 x 4096 20.2 / 15.6 / 13.2. Above that tiles read a's rows less often: 200 x 8192 x 2048 24.8 against 14.6,
+// 32 x 32768 x 4096 32.0 against 26.3; 16 rows or less are so small that they do not count: 16 x 32768 x 4096 22.7
+// against 25.9.
+// Tiles of 256 x 256 cost 8/9 of the four of 128 x 128 that they replace (16384 x 8192 x 4096 550 against 619), but a
+// last turn of few tiles costs more: the CUs' turns decide. 4096 x 4096 x 4096 71 against 81; the other way
+// 2331 x 8192 x 4096 123 against 99, 6000 x 4096 x 4096 126 against 118.
 template <int OUT>
 hipError_t gemm(const F8Gemm& p, int cus, hipStream_t s) {
-    if (p.m <= 64) {
-        const dim3 grid((unsigned)((p.n + 15) / 16)), block(64 * FW);
-        if (p.m <= 16) hipLaunchKernelGGL((gemm_few<OUT, 1>), grid, block, 0, s, p);
-        else if (p.m <= 32) hipLaunchKernelGGL((gemm_few<OUT, 2>), grid, block, 0, s, p);
-        else hipLaunchKernelGGL((gemm_few<OUT, 4>), grid, block, 0, s, p);
-        return hipGetLastError();
-    }
+    hipError_t err = hipSuccess;
+    if (p.m <= 16 && few<OUT, 1>(p, cus, s, err)) return err;
+    if (p.m <= 32 && few<OUT, 2>(p, cus, s, err)) return err;
+    if (few<OUT, 4>(p, cus, s, err)) return err;
     const int64_t big = (((int64_t)p.m + 255) / 256) * (((int64_t)p.n + 255) / 256);
-    if (big >= cus) return tiles<OUT, 256, 256, 2, 4, 2>(p, s);
+    const int64_t mid = (((int64_t)p.m + 127) / 128) * (((int64_t)p.n + 127) / 128);
+    if (32 * ((big + cus - 1) / cus) <= 9 * ((mid + cus - 1) / cus)) return tiles<OUT, 256, 256, 2, 4, 2>(p, s);
     return tiles<OUT, 128, 128, 2, 2, 2>(p, s);
 }
 
