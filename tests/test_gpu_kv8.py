@@ -600,6 +600,109 @@ def test_pool_past_four_gigabytes(ta, gpu_ready):
         assert np.array_equal(got[h], model.block(0, 0, h, 0)[0])
 
 
+# Steps whose rows per K/V head (new tokens times the heads that share it) pass 1024 go through another kernel.
+MANY = [(code, dtype, d) for code in ("e4m3", "i8") for dtype in ("bf16", "f16") for d in (64, 128)]
+
+
+@pytest.mark.parametrize("heads,kv,lens,news", [
+    (24, 1, [130, 1, 64, 63], [130, 1, 60, 0]), (40, 2, [700, 64], [60, 64]), (21, 1, [3000], [50]),
+    (3, 3, [1100, 129], [1090, 65]), (32, 1, [65, 190], [33, 2])])
+@pytest.mark.parametrize("code,dtype,d", MANY)
+def test_many_rows(ta, gpu_ready, code, dtype, d, heads, kv, lens, news):
+    """Prompts, new tokens behind a cache, groups of heads that divide no tile, the keys split and not; scores that
+    keep rising, so that the maximum moves; rows behind the last token stay."""
+    torch = _t()
+    rng = np.random.default_rng(sum(lens) + heads + d)
+    total = sum(news)
+    pool = _pool(ta, len(lens), sum(-(-n // 64) for n in lens), kv, d, code, dtype, 4096, sum(lens) + 3)
+    model = ref.Model(len(lens), kv, d, code, pool.cache.blocks, 64)
+    for n_new in ([n - m for n, m in zip(lens, news)], news):
+        t = sum(n_new)
+        k = _tokens(rng, t, kv, d, dtype) * np.linspace(0.2, 2.0, t)[:, None, None].astype(np.float32)
+        _step(torch, pool, model, n_new, _round(k, dtype), _tokens(rng, t, kv, d, dtype, 30.0), dtype)
+    q = _round(rng.standard_normal((total, heads, d)) * 2, dtype)
+    qd = _dev(np.concatenate([q, np.zeros((3, heads, d), np.float32)]), dtype)
+    for new, length in ((max(news), max(lens)), (0, 0), (max(news), 64)):
+        o = torch.full_like(qd, -7.0)
+        pool.attend(qd, o, d ** -0.5, max_new=new, max_len=length)
+        assert (o[total:] == -7).all()
+        _check_attend(torch, pool, model, news, q, o, d ** -0.5, dtype, kv)
+
+
+@pytest.mark.parametrize("code,dtype,d", MANY)
+def test_many_rows_no_numbers(ta, gpu_ready, code, dtype, d):
+    """As for few rows: a NaN or infinity of a tail's V reaches the rows that read its token, of a block those that read
+    the block, an infinite K of a masked token nothing, a table that names no block its own request."""
+    torch = _t()
+    rng = np.random.default_rng(d)
+    heads, kv, held, news = 48, 2, 70, 50  # tokens 70 .. 119; the tail starts at 64; 1200 rows a K/V head
+    n = held + news
+    q = _round(rng.standard_normal((2 * news, heads, d)), dtype)
+    keep = np.concatenate([np.arange(held), n + np.arange(held)])
+    rest = np.concatenate([np.arange(held, n), n + np.arange(held, n)])
+    k0, v0 = _tokens(rng, 2 * n, kv, d, dtype), _tokens(rng, 2 * n, kv, d, dtype)
+    half = heads // kv
+    for where, bad in (("v", float("nan")), ("v", float("inf")), ("k", -float("inf")), ("k_block", float("nan")),
+                       ("v_block", float("inf")), ("table", 99), ("table", -1)):
+        pool = _pool(ta, 2, 4, kv, d, code, dtype, 128, 2 * n)
+        model = ref.Model(2, kv, d, code, 4, 2)
+        k, v = k0.copy(), v0.copy()
+        tok = 5 if "block" in where else 100  # of request 0, K/V head 1
+        if where != "table":
+            (k if where[0] == "k" else v)[tok, 1, 3] = bad
+        _step(torch, pool, model, [held, held], k[keep], v[keep], dtype)
+        _step(torch, pool, model, [news, news], k[rest], v[rest], dtype)
+        if where == "table":
+            pool.table[0, 0] = bad
+        o = torch.empty((2 * news, heads, d), dtype=_dtype(dtype), device="cuda")
+        pool.attend(_dev(q, dtype), o, d ** -0.5, max_new=news, max_len=n)
+        isnan = torch.isnan(o).any(-1).cpu().numpy()
+        want = np.zeros((2 * news, heads), bool)
+        if where == "table":
+            want[:news] = True
+        elif "block" in where:
+            want[:news, half:] = True
+        else:
+            want[tok - held:news, half:] = True
+        if where == "v" and bad == bad:  # an infinity times a weight is one, or NaN where others meet it
+            isnan |= torch.isinf(o).any(-1).cpu().numpy()
+        if where == "k":  # rows that see it: a weight of 0 (a score of -inf) or NaN; the rows before are checked below
+            isnan[tok - held:news, half:] = True
+        assert np.array_equal(isnan, want), (where, bad)
+        # the rows that do not see it are what they are without it
+        if where in ("v", "k"):
+            (model.v if where == "v" else model.k)[0][tok, 1, 3] = 0
+            a, b, s = ref.attend(q[:tok - held, heads - 1], *model.values(0, 1), held + np.arange(tok - held), d ** -0.5)
+            bound = ref.attend_bound(a, b, s, np.abs(model.values(0, 1)[1]).max(), n, HALF[dtype], dtype == "f16")
+            assert (np.abs(o[:tok - held, heads - 1].float().cpu().numpy() - a) <= bound).all()
+        _check_attend(torch, pool, model, [news, news], q, o, d ** -0.5, dtype, kv, skip=(0,))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_many_rows_of_short_requests(ta, gpu_ready, d):
+    """Counts that do not fit, with many rows: clamped as for few, the rows before a request's start 0."""
+    torch = _t()
+    rng = np.random.default_rng(d)
+    heads, T = 24, 80
+    pool = _pool(ta, 3, 12, 1, d, "e4m3", "bf16", 256, T)
+    model = ref.Model(3, 1, d, "e4m3", 12, 4)
+    k = _tokens(rng, T, 1, d, "bf16")
+    _step(torch, pool, model, [40, 30, 10], k, k, "bf16")
+    q, o = _dev(rng.standard_normal((T, heads, d)), "bf16"), torch.full((T, heads, d), -7.0, dtype=torch.bfloat16, device="cuda")
+    big = (1 << 31) - 1
+    for cu, length in (([0, 1000, 2000, big], [40, 30, 10]), ([-5, 90, 20, 10], [40, 30, 10]),
+                       ([0, 40, 70, 80], [big, 30, 10]), ([0, 40, 70, 80], [-3, 30, 10])):
+        pool.cu_tokens.copy_(torch.tensor(cu, dtype=torch.int32))
+        pool.length.copy_(torch.tensor(length, dtype=torch.int32))
+        pool.attend(q, o, 0.125, max_new=80)
+    pool.cu_tokens.copy_(torch.tensor([0, 40, 70, 80], dtype=torch.int32))
+    pool.length.copy_(torch.tensor([25, 30, 10], dtype=torch.int32))
+    o.fill_(-7)
+    pool.attend(q, o, 0.125, max_new=80)
+    assert (o[:15] == 0).all() and (o[15:40] != 0).any()
+    _check_attend(torch, pool, model, [40, 30, 10], q.float().cpu().numpy(), o, 0.125, "bf16", 1, skip=(0,))
+
+
 def test_refusals_of_the_binding(ta, gpu_ready):
     """What the binding or the call refuses on real tensors: nothing is launched."""
     torch = _t()
