@@ -401,11 +401,16 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(few_wav
 }
 
 // ---- many rows: tiles through LDS ----
-// One workgroup = (request, K/V head, 128 rows, chunk of the keys), four waves of 32 rows on v_mfma_f32_32x32x16. Each
-// cache block is decoded once per workgroup, into LDS in the instructions' operand order, while the waves compute the
-// block before it; its codes are loaded a block earlier still. Lane l of a score block holds one row (l % 32) and keys
-// 8 (i / 4) + 4 (l / 32) + i % 4, i < 16: the order in which V's operand takes them, so the weights go from the scores'
-// registers straight into the second product. Bound by the matrix and vector units together.
+// One workgroup = (request, K/V head, 32 rows a wave, chunk of the keys), on v_mfma_f32_32x32x16. Each cache block is
+// decoded once per workgroup, into LDS in the instructions' operand order; its codes are loaded a block earlier. Lane l of
+// a score block holds one row (l % 32) and keys 8 (i / 4) + 4 (l / 32) + i % 4, i < 16: the order in which V's operand takes
+// them, so the weights go from the scores' registers straight into the second product.
+// A step computes the next block's scores beside this block's exponentials, and this block's second product beside the
+// decoding, one product and a few vector instructions at a time, its operands read from LDS a product ahead (products and
+// vector work one after the other, operands read where they were needed: 555 us where this takes 473, four requests of up
+// to 2048 new tokens over 8192, 32 heads of 128 dims, 8 in the cache; 494 GFLOP). Bound by the issue of two waves a SIMD:
+// each unit is busy 40 to 45 % of the time; without the exponentials it takes 7 % less,
+// without the decoding 14 %, without half of the products 18 %.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 template <bool BF16>
@@ -416,19 +421,22 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-constexpr int MW = 4;           // waves
-constexpr int MROWS = 32 * MW;  // rows of a workgroup (256 at 128 dims: 303 us where these take 273, 16 requests of 512
-                                // tokens and 4 heads a K/V head over 4096)
+// Waves: 8 at 128 dims, one workgroup a CU, decode a block for 256 rows (4: 505 us where these take 485). At 64 dims 4,
+// with two workgroups a CU and 256 registers a lane (three and 168: 281 us where these take 214, 16 requests of 128
+// tokens and 16 heads over up to 4096).
+constexpr int many_waves(int d) { return d == 64 ? 4 : 8; }
 // The running max follows a block's only when it is passed by this much (exp2 units): weights up to 2^8 cost nothing,
 // and O is rescaled a few times per row instead of in every block.
 constexpr float kSlack = 8.f;
 
 template <int CODE, bool BF16, int D>
-__global__ __launch_bounds__(64 * MW) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2))) void attend_many(Kv8Attend p) {
+__global__ __launch_bounds__(64 * many_waves(D)) __attribute__((amdgpu_waves_per_eu(2, 2))) void attend_many(Kv8Attend p) {
+    constexpr int MW = many_waves(D), MROWS = 32 * MW;
     constexpr int KS = D / 16;  // 16-dim steps of a score
     constexpr int DB = D / 32;  // 32-dim blocks of O
     constexpr int U = D / 16 / MW;        // 16-byte pieces of K, and of V, per thread and block
     static_assert(U * MW * 16 == D, "every thread stages as much");
+    constexpr int PS = DB / U;            // a piece of the staging goes with every PS-th of the second products
     // Operand blocks of 1 KB (lane l's 16 bytes at 16 l). K: (32 keys, 16-dim step); V: (16 keys, 32 dims).
     constexpr uint32_t kOp = 1024 + 128;  // 128 bytes apart: a staging wave's pieces of two steps lie on different banks
     constexpr uint32_t kK = 2 * KS * kOp, kStage = kK + 4 * DB * kOp;
@@ -444,7 +452,7 @@ __global__ __launch_bounds__(64 * MW) __attribute__((amdgpu_waves_per_eu(D == 64
     const Kv8& c = p.c;
     // Row tiles of one (request, head, chunk) read the same keys: on one XCD, whose L2 then holds them. Workgroups go to
     // the 8 XCDs in turn, and the triples are dealt to XCDs in turn too, heads first: every XCD has its share of each
-    // request, however their lengths differ (requests dealt to XCDs whole: 999 us where this takes 480). Late tiles,
+    // request, however their lengths differ (requests dealt to XCDs whole: 999 us where this took 581). Late tiles,
     // which read the most keys, first.
     const int idx = blockIdx.x >> 3;
     const int tile0 = p.tiles - 1 - idx % p.tiles;
@@ -485,54 +493,54 @@ __global__ __launch_bounds__(64 * MW) __attribute__((amdgpu_waves_per_eu(D == 64
         // K: a wave's load covers 1 KB: 16 keys of 64 dims (lane: key l % 16, step l / 16) or 8 keys of 128 (key l % 8,
         // step l / 8). V: the thread's dim and 16-byte piece g of its tokens.
         u32x4 kc[U], vc[U];
-        auto load = [&](int blk) {
-            const bool ok = blk >= 0 && blk < c.blocks;
-            const int64_t at = ((int64_t)(ok ? blk : 0) * c.heads + h) * kKvBlock * D;
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int key = D == 64 ? 16 * (U * wave + u) + (lane & 15) : 8 * (U * wave + u) + (lane & 7);
-                const int step = D == 64 ? lane >> 4 : lane >> 3;
-                kc[u] = ld16(c.k + at + key * D + 16 * step);
-                const int dim = 16 * (U * wave + u) + (lane & 15);
-                vc[u] = ld16(c.v + at + dim * kKvBlock + 16 * (lane >> 4));
-            }
+        auto base = [&](int blk) { return ((int64_t)blk * c.heads + h) * kKvBlock * D; };
+        auto load_k = [&](int blk, int u) {
+            const int key = D == 64 ? 16 * (U * wave + u) + (lane & 15) : 8 * (U * wave + u) + (lane & 7);
+            kc[u] = ld16(c.k + base(blk) + key * D + 16 * (D == 64 ? lane >> 4 : lane >> 3));
         };
-        auto stage = [&](int buf) {
-            const uint32_t st = lds0 + buf * kStage;
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int key = D == 64 ? 16 * (U * wave + u) + (lane & 15) : 8 * (U * wave + u) + (lane & 7);
-                const int step = D == 64 ? lane >> 4 : lane >> 3;
-                const uint32_t a = st + ((key >> 5) * KS + step) * kOp + 16 * (key & 31);
-                *(lds_u32x4_ptr)(uintptr_t)a = decode8<CODE, BF16>(kc[u][0], kc[u][1]);
-                *(lds_u32x4_ptr)(uintptr_t)(a + 512) = decode8<CODE, BF16>(kc[u][2], kc[u][3]);
-                // V: words (c2, a2) of piece g are tokens 16 (2 c2 + a2) + 4 g .. + 3: four of the operand's eight slots
-                const int dim = 16 * (U * wave + u) + (lane & 15), g = lane >> 4;
-                const uint32_t b = st + kK + (dim >> 5) * kOp + 16 * (32 * (g & 1) + (dim & 31)) + 8 * (g >> 1);
-                const u32x4 lo = decode8<CODE, BF16>(vc[u][0], vc[u][1]), hi = decode8<CODE, BF16>(vc[u][2], vc[u][3]);
-                *(lds_u32x2_ptr)(uintptr_t)(b) = u32x2{lo[0], lo[1]};
-                *(lds_u32x2_ptr)(uintptr_t)(b + DB * kOp) = u32x2{lo[2], lo[3]};
-                *(lds_u32x2_ptr)(uintptr_t)(b + 2 * DB * kOp) = u32x2{hi[0], hi[1]};
-                *(lds_u32x2_ptr)(uintptr_t)(b + 3 * DB * kOp) = u32x2{hi[2], hi[3]};
-            }
+        auto load_v = [&](int blk, int u) {
+            vc[u] = ld16(c.v + base(blk) + (16 * (U * wave + u) + (lane & 15)) * kKvBlock + 16 * (lane >> 4));
+        };
+        auto stage_k = [&](int buf, int u, int half) {
+            const int key = D == 64 ? 16 * (U * wave + u) + (lane & 15) : 8 * (U * wave + u) + (lane & 7);
+            const int step = D == 64 ? lane >> 4 : lane >> 3;
+            const uint32_t a = lds0 + buf * kStage + ((key >> 5) * KS + step) * kOp + 16 * (key & 31);
+            *(lds_u32x4_ptr)(uintptr_t)(a + 512 * half) = decode8<CODE, BF16>(kc[u][2 * half], kc[u][2 * half + 1]);
+        };
+        auto stage_v = [&](int buf, int u, int half) {
+            // Words (c2, a2) of piece g are tokens 16 (2 c2 + a2) + 4 g .. + 3: four of the operand's eight slots.
+            const int dim = 16 * (U * wave + u) + (lane & 15), g = lane >> 4;
+            const uint32_t b = lds0 + buf * kStage + kK + (dim >> 5) * kOp + 16 * (32 * (g & 1) + (dim & 31)) + 8 * (g >> 1);
+            const u32x4 x = decode8<CODE, BF16>(vc[u][2 * half], vc[u][2 * half + 1]);
+            *(lds_u32x2_ptr)(uintptr_t)(b + 2 * half * DB * kOp) = u32x2{x[0], x[1]};
+            *(lds_u32x2_ptr)(uintptr_t)(b + (2 * half + 1) * DB * kOp) = u32x2{x[2], x[3]};
         };
         // The tail's values as they are; rows past the last token 0. V's that are no numbers: 0, and their keys noted.
-        auto stage_tail = [&](int buf) {
+        auto tail_k = [&](int buf) {
             int tid_t = tid;  // opaque: its addresses are not kept across the loop
             asm volatile("" : "+v"(tid_t));
-            const uint32_t st = lds0 + buf * kStage;
             const int live = s.total - nfull * kKvBlock;
             const int64_t at = ((int64_t)r * c.heads + h) * kKvBlock * D;
 #pragma unroll 1
             for (int i = tid_t; i < kKvBlock * D / 8; i += 64 * MW) {
                 const int key = i / (D / 8), d0 = 8 * (i % (D / 8));
-                const u32x4 z = {0, 0, 0, 0};
-                const u32x4 x = key < live ? ld16(c.k_tail + at + key * D + d0) : z;
-                *(lds_u32x4_ptr)(uintptr_t)(st + ((key >> 5) * KS + (d0 >> 4)) * kOp + 16 * (32 * ((d0 >> 3) & 1) + (key & 31))) = x;
-                const u32x4 y = key < live ? ld16(c.v_tail + at + key * D + d0) : z;
+                *(lds_u32x4_ptr)(uintptr_t)(lds0 + buf * kStage + ((key >> 5) * KS + (d0 >> 4)) * kOp +
+                                            16 * (32 * ((d0 >> 3) & 1) + (key & 31))) =
+                    key < live ? ld16(c.k_tail + at + key * D + d0) : u32x4{0, 0, 0, 0};
+            }
+        };
+        auto tail_v = [&](int buf) {
+            int tid_t = tid;
+            asm volatile("" : "+v"(tid_t));
+            const int live = s.total - nfull * kKvBlock;
+            const int64_t at = ((int64_t)r * c.heads + h) * kKvBlock * D;
+#pragma unroll 1
+            for (int i = tid_t; i < kKvBlock * D / 8; i += 64 * MW) {
+                const int key = i / (D / 8), d0 = 8 * (i % (D / 8));
+                const u32x4 y = key < live ? ld16(c.v_tail + at + key * D + d0) : u32x4{0, 0, 0, 0};
                 const int slot = key & 15;  // of its 16 keys: lane half (slot / 4) % 2, element 4 (slot / 8) + slot % 4
-                const uint32_t b = st + kK + ((key >> 4) * DB + (d0 >> 5)) * kOp + 16 * (32 * ((slot >> 2) & 1) + (d0 & 31)) +
-                                   2 * (4 * (slot >> 3) + (slot & 3));
+                const uint32_t b = lds0 + buf * kStage + kK + ((key >> 4) * DB + (d0 >> 5)) * kOp +
+                                   16 * (32 * ((slot >> 2) & 1) + (d0 & 31)) + 2 * (4 * (slot >> 3) + (slot & 3));
                 bool any = false;
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
@@ -548,20 +556,90 @@ __global__ __launch_bounds__(64 * MW) __attribute__((amdgpu_waves_per_eu(D == 64
             }
         };
 
-        // ---- one block ----
-        auto compute = [&](int j, int buf, float kx, float lv, bool tail) {
-            const int k0 = j * kKvBlock;
+        // ---- the blocks, one score product ahead ----
+        // K of block j is in buffer j - b0, V too, both mod 2. At the start of step j: K up to block j + 1 and V up to j in
+        // LDS, block j + 2's K codes and j + 1's V codes in registers. Past the last whole block old codes are staged again,
+        // which nothing reads: the step stays free of branches.
+        // Table entries and scales of 64 blocks at a time, a block per lane; a step takes its own from there.
+        struct Block {
+            int id;
+            float sk, sv;
+        };
+        int lane_id = 0;
+        f32x2 lane_s = {0, 0};
+        auto block = [&](int x) {  // the chunk's x-th; the last whole one past the end
+            if ((x & 63) == 0) {
+                const int blk = table[max(0, min(b0 + x + lane, bq - 1))];
+                const bool ok = blk >= 0 && blk < c.blocks;
+                lane_id = ok ? blk : 0;
+                lane_s = ld2(c.scales + 2 * ((int64_t)lane_id * c.heads + h));
+                if (!ok) lane_s[0] = __builtin_nanf("");
+                float sk = lane_s[0], sv = lane_s[1];
+                asm volatile("" : "+v"(sk), "+v"(sv));  // waited for here, not with the codes' loads behind the branch
+                lane_s = f32x2{sk, sv};
+            }
+            return Block{__builtin_amdgcn_readlane(lane_id, x & 63),
+                         __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lane_s[0]), x & 63)),
+                         __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lane_s[1]), x & 63))};
+        };
+        auto operand = [&](int buf, int i) { return *(lds_u32x4_ptr)(uintptr_t)(lds0 + buf * kStage + 16 * lane + i * kOp); };
+        Block n0 = block(0), n1 = block(1), n2 = block(2), n3 = block(3);  // blocks j .. j + 3
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            load_k(n0.id, u);
+            load_v(n0.id, u);
+        }
+        if (tid == 0) bad_keys = 0;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            stage_k(0, u, 0);
+            stage_k(0, u, 1);
+            load_k(n1.id, u);
+            stage_v(0, u, 0);
+            stage_v(0, u, 1);
+            load_v(n1.id, u);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            stage_k(1, u, 0);
+            stage_k(1, u, 1);
+            load_k(n2.id, u);
+        }
+        __syncthreads();
+        if (b0 >= nfull) {
+            tail_k(0);
+            __syncthreads();
+        }
+        f32x16 s_even[2], s_odd[2];
+#pragma unroll
+        for (int t = 0; t < KS; t++)
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+                s_even[kb] = mfma32<BF16>(operand(0, kb * KS + t), qf[t], t == 0 ? f32x16{} : s_even[kb]);
+        __syncthreads();  // block b0's K is overwritten in the first step
+
+        float mx[2];  // of the scores' products, as they are: half a row's keys each
+        auto top = [&](f32x16 (&sb)[2], int first, int end) {
+#pragma unroll
+            for (int i = first; i < end; i++) {
+                mx[0] = i ? fmaxf(mx[0], sb[0][i]) : sb[0][0];
+                mx[1] = i ? fmaxf(mx[1], sb[1][i]) : sb[1][0];
+            }
+        };
+        top(s_even, 0, 16);
+
+        auto step = [&](int j, int buf, f32x16 (&sb)[2], f32x16 (&next)[2]) {
+            const bool tail = j >= nfull;
+            if (j + 1 == nfull || tail) {  // the tail is the last block there is
+                if (tail) tail_v(buf);
+                else if (j + 1 < b1) tail_k(buf ^ 1);
+                __syncthreads();
+            }
+            u32x4 kop[2] = {operand(buf ^ 1, 0), operand(buf ^ 1, KS)}, vop[DB];  // read a group of products ahead
+            float kx = tail ? p.c2 : n0.sk * p.c2, lv = tail ? 0.f : __builtin_amdgcn_logf(n0.sv);
             const float inv_v = __builtin_amdgcn_exp2f(-lv);
-            const uint32_t st = lds0 + buf * kStage + 16 * lane;
-            f32x16 sb[2] = {f32x16{}, f32x16{}};
-#pragma unroll
-            for (int t = 0; t < KS; t++)  // two independent chains: an instruction's result is twice its issue away
-#pragma unroll
-                for (int kb = 0; kb < 2; kb++)
-                    sb[kb] = mfma32<BF16>(*(lds_u32x4_ptr)(uintptr_t)(st + (kb * KS + t) * kOp), qf[t], sb[kb]);
-            __builtin_amdgcn_sched_barrier(0);
-            if (k0 + kKvBlock > plain_end) {
-                const int rel = kv_end - k0 - 4 * lh;  // register i's key is seen where its offset is below
+            if ((j + 1) * kKvBlock > plain_end) {
+                const int rel = kv_end - j * kKvBlock - 4 * lh;  // register i's key is seen where its offset is below
 #pragma unroll
                 for (int kb = 0; kb < 2; kb++)
 #pragma unroll
@@ -571,21 +649,16 @@ __global__ __launch_bounds__(64 * MW) __attribute__((amdgpu_waves_per_eu(D == 64
                     }
                 kx = 1.f;  // already applied
                 lv = 0.f;
-            }
-            if (tail && bad_keys != 0) {  // rows that see a key whose V is no number
+                if (tail && bad_keys != 0) {  // rows that see a key whose V is no number
 #pragma unroll
-                for (int kb = 0; kb < 2; kb++) {
-                    const uint32_t w = (uint32_t)(bad_keys >> (32 * kb)) >> (4 * lh);
+                    for (int kb = 0; kb < 2; kb++) {
+                        const uint32_t w = (uint32_t)(bad_keys >> (32 * kb)) >> (4 * lh);
 #pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        if ((w & (1u << (8 * (i >> 2) + (i & 3)))) && sb[kb][i] != kNegInf) sb[kb][i] = __builtin_nanf("");
+                        for (int i = 0; i < 16; i++)
+                            if ((w & (1u << (8 * (i >> 2) + (i & 3)))) && sb[kb][i] != kNegInf) sb[kb][i] = __builtin_nanf("");
+                    }
                 }
-            }
-            float mx[2] = {sb[0][0], sb[1][0]};
-#pragma unroll
-            for (int i = 1; i < 16; i++) {
-                mx[0] = fmaxf(mx[0], sb[0][i]);
-                mx[1] = fmaxf(mx[1], sb[1][i]);
+                top(sb, 0, 16);
             }
             float mloc = __builtin_fmaf(fmaxf(mx[0], mx[1]), kx, lv);
             const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mloc), __float_as_uint(mloc), false, false);
@@ -605,55 +678,68 @@ __global__ __launch_bounds__(64 * MW) __attribute__((amdgpu_waves_per_eu(D == 64
             }
             const float off = lv - (m_run == kNegInf ? 0.f : m_run);
             u32x4 pf[4];
-            float sum[2] = {0.f, 0.f};
+            // Exponentials in a row, G pairs of them after every second product, and what they need and feed after the others:
+            // each change between them and other vector instructions costs several cycles.
+            constexpr int G = 16 / KS;
+            float sum[2] = {0.f, 0.f}, w[2][2 * G];
+            auto add = [&](int g) {
 #pragma unroll
-            for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sb[kb][i], kx, off));
-                    const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sb[kb][i + 1], kx, off));
+                for (int e = 0; e < G; e++) {
+                    const float e0 = w[g & 1][2 * e], e1 = w[g & 1][2 * e + 1];
                     sum[0] += e0;
                     sum[1] += e1;
-                    pf[2 * kb + (i >> 3)][(i & 7) >> 1] = pack2<BF16>(e0, e1);
+                    pf[(g * G + e) >> 2][(g * G + e) & 3] = pack2<BF16>(e0, e1);
                 }
+            };
+#pragma unroll
+            for (int n = 0; n < 2 * KS; n++) {
+                const int t = n >> 1, kb = n & 1;
+                next[kb] = mfma32<BF16>(kop[kb], qf[t], t == 0 ? f32x16{} : next[kb]);
+                if (t + 1 < KS) kop[kb] = operand(buf ^ 1, kb * KS + t + 1);
+                if (n + 1 == 2 * KS)
+#pragma unroll
+                    for (int db = 0; db < DB; db++) vop[db] = operand(buf, 2 * KS + db);
+                __builtin_amdgcn_sched_barrier(0);
+                if (kb == 0 && t > 0) add(t - 1);
+#pragma unroll
+                for (int e = 0; e < 2 * G; e++) {
+                    const int x = 2 * G * t + e;
+                    w[t & 1][e] = kb == 0 ? __builtin_fmaf(sb[x >> 4][x & 15], kx, off) : __builtin_amdgcn_exp2f(w[t & 1][e]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            add(KS - 1);
             l_run = __builtin_fmaf(sum[0] + sum[1], inv_v, l_run);
 #pragma unroll
-            for (int q = 0; q < 4; q++)
-#pragma unroll
-                for (int db = 0; db < DB; db++)
-                    oacc[db] = mfma32<BF16>(*(lds_u32x4_ptr)(uintptr_t)(st + kK + (q * DB + db) * kOp), pf[q], oacc[db]);
-        };
-
-        if (tid == 0) bad_keys = 0;
-        __syncthreads();
-        float2 sc = {1.f, 1.f}, sc_next = sc;  // the scales of the block in LDS, and of the one in registers
-        int blk_next = b0 < bq ? table[b0] : 0;  // the table's entry for the block to load next: read a block ahead
-        auto fetch = [&](int j) {
-            const int blk = blk_next;
-            load(blk);
-            sc_next = reinterpret_cast<const float2*>(c.scales)[(int64_t)(blk >= 0 && blk < c.blocks ? blk : 0) * c.heads + h];
-            if (blk < 0 || blk >= c.blocks) sc_next.x = __builtin_nanf("");
-            if (j + 1 < bq) blk_next = table[j + 1];
-        };
-        auto advance = [&](int j, int buf) {  // block j into LDS, block j + 1 into registers
-            if (j < bq) {
-                stage(buf);
-                sc = sc_next;
-                if (j + 1 < bq) fetch(j + 1);
-            } else if (j < b1) {
-                stage_tail(buf);
+            for (int n = 0; n < 4 * DB; n++) {
+                const int q = n / DB, db = n % DB;
+                oacc[db] = mfma32<BF16>(vop[db], pf[q], oacc[db]);
+                if (q < 3) vop[db] = operand(buf, 2 * KS + (q + 1) * DB + db);
+                __builtin_amdgcn_sched_barrier(0);
+                if (n & 1) {
+                    top(next, 8 / DB * (n >> 1), 8 / DB * (n >> 1) + 8 / DB);
+                    asm volatile("" : "+v"(mx[0]), "+v"(mx[1]));  // here, not at its use
+                } else if (n % PS == 0) {
+                    const int i = n / PS, u = i >> 2, half = i & 1;
+                    if (i & 2) stage_v(buf ^ 1, u, half);
+                    else stage_k(buf, u, half);
+                    if (half == 1) {
+                        if (i & 2) load_v(n2.id, u);
+                        else load_k(n3.id, u);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-        };
-        if (b0 < bq) fetch(b0);
-        advance(b0, 0);
-        __syncthreads();
-        for (int j = b0; j < b1; j++) {
-            const int buf = (j - b0) & 1;
-            const bool tail = j >= nfull;
-            const float kx = tail ? p.c2 : sc.x * p.c2, lv = tail ? 0.f : __builtin_amdgcn_logf(sc.y);
-            advance(j + 1, buf ^ 1);
-            compute(j, buf, kx, lv, tail);
+            n0 = n1;
+            n1 = n2;
+            n2 = n3;
+            n3 = block(j + 4 - b0);
             __syncthreads();
+        };
+        for (int j = b0; j < b1; j += 2) {
+            step(j, 0, s_even, s_odd);
+            if (j + 1 == b1) break;
+            step(j + 1, 1, s_odd, s_even);
         }
 
         // ---- results ----
@@ -766,7 +852,7 @@ hipError_t attend(const Kv8Attend& p, hipStream_t s) {
     const dim3 g((unsigned)grid), b(64 * NW);
     if (p.kernel == kAttendMany) {
         const int64_t eights = ((int64_t)p.c.requests * p.c.heads * p.chunks + 7) / 8;  // of (request, head, chunk)
-        hipLaunchKernelGGL((attend_many<CODE, BF16, D>), dim3((unsigned)(eights * 8 * p.tiles)), dim3(64 * MW), 0, s, p);
+        hipLaunchKernelGGL((attend_many<CODE, BF16, D>), dim3((unsigned)(eights * 8 * p.tiles)), dim3(64 * many_waves(D)), 0, s, p);
     }
     else if (p.rows == 16 && p.once) hipLaunchKernelGGL((attend_few<CODE, BF16, D, 1, true>), g, b, 0, s, p);
     else if (p.rows == 16) hipLaunchKernelGGL((attend_few<CODE, BF16, D, 1, false>), g, b, 0, s, p);
@@ -794,11 +880,14 @@ int64_t kv8_attend_plan(Kv8Attend& p, int head_dim, int max_new, int max_len, in
     const int64_t len = max_len > 0 && max_len < most ? max_len : most;
     const int64_t fresh = max_new > 0 && max_new < p.max_tokens ? max_new : p.max_tokens;
     const int64_t rows = fresh * p.group;
-    // Whole tiles through LDS pay where there are many rows to share a block's decoding (us, tiles of 128 rows / of 32; four
-    // requests of up to 4096 tokens, 64 dims: 512 rows 69 / 42, 1024 84 / 66, 2048 95 / 103; 128 dims 57 / 44, 88 / 68,
-    // 119 / 122; 1200 rows over 20000 tokens 138 / 219; four prompts of up to 8192 rows over 8192 tokens 551 / 749).
+    // Whole tiles through LDS pay where there are many rows to share a block's decoding (us, tiles of 128 or 256 rows / of
+    // 32; four requests of up to 4096 tokens, 64 dims: 512 rows 59 / 40, 1024 58 / 65, 2048 81 / 103; 128 dims 48 / 42,
+    // 74 / 67, 107 / 122; one request 1024 rows 44 / 35 and 37 / 42, 16 173 / 162 and 190 / 171; 1200 rows over 20000 tokens
+    // 123 / 219; four prompts of up to 8192 rows over 8192 tokens 473 / 749).
     p.kernel = rows <= 1024 ? kAttendFew : kAttendMany;
-    p.rows = p.kernel == kAttendMany ? MROWS : rows <= 16 ? 16 : 32;
+    p.rows = p.kernel == kAttendMany ? 32 * many_waves(head_dim) : rows <= 16 ? 16 : 32;
+    // A cache too large to stay in the last-level cache is read past it: loads marked as used once (545 MB of K and V 106 ->
+    // 96 us; the other way, 69 MB 20.0 -> 20.4 and 34 MB in blocks of 32 tokens 29.7 -> 33.8).
     p.once = (int64_t)p.c.requests * len * p.c.heads * head_dim >= (int64_t)256 << 20;
     const int64_t tiles = (rows + p.rows - 1) / p.rows;
     p.tiles = (int32_t)(tiles < 1024 ? tiles : 1024);
@@ -808,7 +897,7 @@ int64_t kv8_attend_plan(Kv8Attend& p, int head_dim, int max_new, int max_len, in
     // (two requests of 262144 tokens, 8 heads of 128: 384 workgroups 134 us, 768 147, 1536 163; 32 requests of up to
     // 2048 tokens, 16 heads of 64: unsplit 18.3 us, in two with the join 20.2). Chunks are 8 to 128 blocks: shorter ones
     // are all start and merge, and a longer one would keep a single workgroup busy after the others.
-    const int64_t chunks_wanted = std::max<int64_t>(1, (int64_t)cus * (p.kernel == kAttendMany ? 2 : few_waves(head_dim, p.rows / 16)) / base);
+    const int64_t chunks_wanted = std::max<int64_t>(1, (int64_t)cus * (p.kernel == kAttendMany ? head_dim == 64 ? 2 : 1 : few_waves(head_dim, p.rows / 16)) / base);
     const int64_t chunk = std::min<int64_t>(128, std::max<int64_t>(8, (blocks + chunks_wanted - 1) / chunks_wanted));
     const int64_t chunks = (blocks + chunk - 1) / chunk;
     p.chunk = (int32_t)chunk;
