@@ -284,11 +284,13 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(OC
     // Pieces are swizzled by half the row: 16 lanes, which LDS serves together, read two rows a bank half and eight
     // places in each. (By the row itself: every read two deep on its banks.)
     static_assert(AI % 2 == 0 && BI % 2 == 0, "the swizzle's upper bit goes by the instruction's parity");
-    const int srow = lane >> 3, spiece = (lane & 7) ^ (srow >> 1);
-    const uint32_t a_off = (uint32_t)(wave * AI * 8 + srow) * (uint32_t)p.a_ld;
-    const uint32_t b_off = (uint32_t)(wave * BI * 8 + srow) * (uint32_t)p.b_ld;
+    const int srow = lane >> 3, spiece0 = (lane & 7) ^ (srow >> 1);
+    const uint32_t a_off0 = (uint32_t)(wave * AI * 8 + srow) * (uint32_t)p.a_ld;
+    const uint32_t b_off0 = (uint32_t)(wave * BI * 8 + srow) * (uint32_t)p.b_ld;
     auto stage = [&](int kb, int buf) {
         const uint32_t st = lds0 + buf * kStage;
+        uint32_t a_off = a_off0, b_off = b_off0, spiece = spiece0;
+        asm volatile("" : "+v"(a_off), "+v"(b_off), "+v"(spiece));  // else every address is kept over the loop
 #pragma unroll
         for (int i = 0; i < AI; i++) {
             const uint32_t at = 16u * (spiece ^ (4 * (i & 1)));
@@ -316,53 +318,71 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(OC
         for (int j = 0; j < NT; j++) acc[i][j] = f32x16{};
     // The scales' products, by step, row and 128 columns, in LDS: a thread keeps one row and column group, four steps at a
     // time (16-byte loads; a load per step, wave and row asked for sixteen times as many cache lines). Steps k and k + 8
-    // share a place. Loads and writes come before the step's copies: the wait for them would wait for those too.
-    const int sgrp = threadIdx.x / TM;
-    const bool scaler = sgrp < TN / KB;  // whole waves
-    const float* const sa = p.a_scales + (int64_t)min(m0 + (int)(threadIdx.x % TM), p.m - 1) * p.a_scales_ld;
-    const float* const sb = p.b_scales + (int64_t)min(n0 / KB + min(sgrp, TN / KB - 1), (p.n - 1) / KB) * p.b_scales_ld;
+    // share a place. At step kb: fetched where kb % 4 is 0, written for the next four where it is 3; at the end some again.
     typedef f32x4 f32x4_any __attribute__((aligned(4)));
-    auto put = [&](int k, float v) { scales[k & 7][sgrp][threadIdx.x % TM] = v; };
     f32x4 va = {0, 0, 0, 0}, vb = va;
-    if (scaler)
-        for (int k = 0; k < min(4, kbs); k++) put(k, sa[k] * sb[k]);
-    stage(0, 0);
-    for (int kb = 0; kb < kbs; kb++) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        const int ahead = min((kb & ~3) + 4, kbs - 4);  // steps whose scales are fetched now; at the end some again
-        if (scaler && (kb | 3) + 1 < kbs) {
-            if ((kb & 3) == 0) {
-                va = *reinterpret_cast<const f32x4_any*>(sa + ahead);
-                vb = *reinterpret_cast<const f32x4_any*>(sb + ahead);
-            }
-            if ((kb & 3) == 3)
+    auto fetch_scales = [&](int kb) {
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));  // its addresses are not kept across the loop
+        const int grp = tid / TM, ahead = min((kb & ~3) + 4, kbs - 4);
+        if (grp >= TN / KB || (kb >= 0 && (kb | 3) + 1 >= kbs)) return;  // whole waves
+        const float* const sa = p.a_scales + (int64_t)min(m0 + tid % TM, p.m - 1) * p.a_scales_ld;
+        const float* const sb = p.b_scales + (int64_t)min(n0 / KB + grp, (p.n - 1) / KB) * p.b_scales_ld;
+        if (kb < 0) {  // before the first step: the first four
+            for (int k = 0; k < min(4, kbs); k++) scales[k][grp][tid % TM] = sa[k] * sb[k];
+        } else if ((kb & 3) == 0) {
+            va = *reinterpret_cast<const f32x4_any*>(sa + ahead);
+            vb = *reinterpret_cast<const f32x4_any*>(sb + ahead);
+        } else if ((kb & 3) == 3) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) put(ahead + i, va[i] * vb[i]);
+            for (int i = 0; i < 4; i++) scales[(ahead + i) & 7][grp][tid % TM] = va[i] * vb[i];
         }
-        if (kb + 1 < kbs) stage(kb + 1, (kb + 1) & 1);
-        float s[MT];
+    };
+    fetch_scales(-1);
+    const uint32_t ra = lds0 + wm * KB, rb = lds0 + (TM + wn) * KB;
+    stage(0, 0);
+    if constexpr (OUT != 0) {
+        // Tile by tile, the products of one issued before the multiply-adds of the one before: the vector unit works on
+        // those while the matrix unit is at the next. a's operands are read a tile row ahead, the next step's first ones
+        // beside the last row. The barrier stands before that row, when the wave has read all of this step's data: behind
+        // it the next step's are there, and those of the step after it are sent for into this step's place (the barrier
+        // between steps: 547 us where this takes 526, 16384 x 8192 x 4096). Bound by the matrix unit's share of the wave's
+        // time: 64 of its cycles a product and wave, two waves a SIMD, are 43 % of it.
+        static_assert(MT % 2 == 0, "a tile row's operands and the next one's alternate");
+        Operand<false> a[2][2], b[NT][2];
+        f32x16 x[2];
+        auto read_a = [&](int i, int slot, int buf) {
 #pragma unroll
-        for (int i = 0; i < MT; i++) s[i] = scales[kb & 7][wn / KB][wm + 32 * i + lr];
-        const uint32_t st = lds0 + (kb & 1) * kStage, ra = st + wm * KB, rb = st + (TM + wn) * KB;
-        if constexpr (OUT != 0) {
-            // Tile by tile, the products of one issued before the multiply-adds of the one before: the vector unit works on
-            // those while the matrix unit is at the next. a's operands are read a tile row ahead.
-            Operand<false> b[NT][2], a[2][2];
+            for (int h = 0; h < 2; h++) a[slot][h].set(operand(ra + buf * kStage + 32 * i * KB, h));
+        };
+        auto read_b = [&](int j, int buf) {
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                a[0][h].set(operand(ra, h));
+            for (int h = 0; h < 2; h++) b[j][h].set(operand(rb + buf * kStage + 32 * j * KB, h));
+        };
+        stage(1, 1);  // past k: zeros
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(AI + BI) : "memory");
+        read_a(0, 0, 0);
 #pragma unroll
-                for (int j = 0; j < NT; j++) b[j][h].set(operand(rb + 32 * j * KB, h));
-            }
-            f32x16 x[2];
+        for (int j = 0; j < NT; j++) read_b(j, 0);
+        for (int kb = 0; kb < kbs; kb++) {
+            const int buf = kb & 1;
+            fetch_scales(kb);
+            float s[MT];
+#pragma unroll
+            for (int i = 0; i < MT; i++) s[i] = scales[kb & 7][wn / KB][wm + 32 * i + lr];
 #pragma unroll
             for (int t = 0; t <= MT * NT; t++) {
                 const int i = t / NT, j = t % NT;
+                if (t == (MT - 1) * NT) {
+                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                    asm volatile("" : "+v"(va), "+v"(vb));  // the scales on their way, too, are there
+                    stage(kb + 2, buf);
+                }
                 if (t < MT * NT) {
-                    if (j == 0 && i + 1 < MT)
-#pragma unroll
-                        for (int h = 0; h < 2; h++) a[(i + 1) & 1][h].set(operand(ra + 32 * (i + 1) * KB, h));
+                    if (j == 0) i + 1 < MT ? read_a(i + 1, (i + 1) & 1, buf) : read_a(0, 0, buf ^ 1);
                     x[t & 1] = mul(b[j][1], a[i & 1][1], mul(b[j][0], a[i & 1][0], f32x16{}));
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (i + 1 == MT) read_b(j, buf ^ 1);  // after the last step: nothing's
                 }
                 if (t > 0) {
                     const int u = t - 1;
@@ -372,16 +392,26 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(OC
                 }
                 __builtin_amdgcn_sched_barrier(0x100);  // in this order but for the reads of LDS
             }
-        } else {
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // of the zeros past k
+    } else {
+        for (int kb = 0; kb < kbs; kb++) {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            fetch_scales(kb);  // before the copies: a wait for these would wait for those too
+            if (kb + 1 < kbs) stage(kb + 1, (kb + 1) & 1);
+            float s[MT];
+#pragma unroll
+            for (int i = 0; i < MT; i++) s[i] = scales[kb & 7][wn / KB][wm + 32 * i + lr];
+            const uint32_t at = (kb & 1) * kStage;
 #pragma unroll
             for (int h = 0; h < 2; h++) {  // half a step at a time: f16 operands are twice as large
                 Operand<true> b[NT];
 #pragma unroll
-                for (int j = 0; j < NT; j++) b[j].set(operand(rb + 32 * j * KB, h));
+                for (int j = 0; j < NT; j++) b[j].set(operand(rb + at + 32 * j * KB, h));
 #pragma unroll
                 for (int i = 0; i < MT; i++) {
                     Operand<true> a;
-                    a.set(operand(ra + 32 * i * KB, h));
+                    a.set(operand(ra + at + 32 * i * KB, h));
 #pragma unroll
                     for (int j = 0; j < NT; j++) {
                         const f32x16 x = mul(b[j], a, f32x16{});
@@ -472,7 +502,7 @@ bool few(const F8Gemm& p, int cus, hipStream_t s, hipError_t& err) {
 // 16 x 16384 x 4096 20.2 / 15.6 / 13.2. Above that tiles read a's rows less often: 200 x 8192 x 2048 24.8 against 14.6,
 // 32 x 32768 x 4096 32.0 against 26.3; 16 rows or less are so small that they do not count: 16 x 32768 x 4096 22.7
 // against 25.9.
-// Tiles of 256 x 256 cost 8/9 of the four of 128 x 128 that they replace (16384 x 8192 x 4096 550 against 619), but a
+// Tiles of 256 x 256 cost 8/9 of the four of 128 x 128 that they replace (16384 x 8192 x 4096 547 against 619), but a
 // last turn of few tiles costs more: the CUs' turns decide. 4096 x 4096 x 4096 71 against 81; the other way
 // 2331 x 8192 x 4096 123 against 99, 6000 x 4096 x 4096 126 against 118.
 template <int OUT>
