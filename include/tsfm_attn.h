@@ -804,8 +804,9 @@ typedef struct tsfm_f8_quantize_args {
 int tsfm_f8_quantize(const tsfm_f8_quantize_args *args);
 
 /* c[m, n] = sum over blocks b of 128 of a_scales[m, b] * b_scales[n / 128, b] * (a[m, :] . b[n, :] over the block),
- * a (m, k) and b (n, k) e4m3 codes row-major, products and sums in f32, rounded once to out_dtype. k a
- * multiple of 16; m, n any. Scales of any value. */
+ * a (m, k) and b (n, k) e4m3 codes row-major, sums in f32, rounded once to out_dtype. For 16-bit results the
+ * products of a block are the 8-bit matrix instruction's, which keeps about 2^-17 of the largest of them; for f32
+ * they are exact. k a multiple of 16; m, n any. Scales of any value. */
 typedef struct tsfm_f8_gemm_args {
     int32_t m, n, k;
     int32_t out_dtype;    /* TSFM_DTYPE_* */
