@@ -576,6 +576,34 @@ def test_captured_steps(ta, gpu_ready):
             assert torch.equal(p.slots, eager.slots) and torch.equal(p.status, eager.status)
 
 
+def test_pool_keeps_its_workspace_on_other_streams(ta, gpu_ready, monkeypatch):
+    """Split contexts without a caller's workspace: the pool's grows from call to call and from stream to stream, the
+    memory that it lets go is not handed out while a call still uses it; a capture without one is refused."""
+    torch = _t()
+    rng = np.random.default_rng(53)
+    kv, heads, d, dtype, n = 1, 4, 64, "bf16", 2000
+    pool = _pool(ta, 1, 40, kv, d, "e4m3", dtype, 2560, 2000)
+    model = ref.Model(1, kv, d, "e4m3", 40, 40)
+    _step(torch, pool, model, [n], _tokens(rng, n, kv, d, dtype), _tokens(rng, n, kv, d, dtype), dtype)
+    side = torch.cuda.Stream()
+    for rows, stream in ((1, None), (4, side), (8, side.cuda_stream), (16, None), (24, side), (2, torch.cuda.default_stream())):
+        q = _dev(rng.standard_normal((rows, heads, d)), dtype)
+        pool.cu_tokens.copy_(torch.tensor([0, rows], dtype=torch.int32))
+        hints = dict(max_new=rows, max_len=n)
+        need = ta.kv8_attend_workspace(pool.cache, heads, rows, **hints)
+        assert need > 0
+        o, w = torch.empty_like(q), torch.empty_like(q)
+        pool.attend(q, w, 0.125, workspace=torch.empty(need, dtype=torch.uint8, device="cuda"), **hints)
+        torch.cuda.synchronize()
+        pool.attend(q, o, 0.125, stream=stream, **hints)
+        torch.full((1 << 20,), 7, dtype=torch.uint8, device="cuda")  # takes memory that is free
+        torch.cuda.synchronize()
+        assert torch.equal(o, w), rows
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(ValueError):
+        pool.attend(q, o, 0.125, **hints)
+
+
 def test_pool_past_four_gigabytes(ta, gpu_ready):
     """Blocks whose bytes lie past 2^32 of K and V."""
     torch = _t()

@@ -176,7 +176,7 @@ __global__ __launch_bounds__(64 * FW) void gemm_few(F8Gemm p) {
     __shared__ __attribute__((aligned(16))) float part[FW][MT * NT][64][4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ql = lane & 15, g = lane >> 4;
-    const int mt_n = (p.m + 16 * MT - 1) / (16 * MT), kbs = (p.k + KB - 1) / KB;
+    const int mt_n = (p.m - 1) / (16 * MT) + 1, kbs = (p.k + KB - 1) / KB;
     const int id = xcd_remap(blockIdx.x, gridDim.x);
     const int m0 = id % mt_n * 16 * MT, n0 = id / mt_n * 16 * NT;
     static_assert(KB % (16 * NT) == 0, "b's rows share their scales");
@@ -265,7 +265,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(OC
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lr = lane & 31, lh = lane >> 5;
-    const int mt_n = (p.m + TM - 1) / TM, nt_n = (p.n + TN - 1) / TN;
+    const int mt_n = (p.m - 1) / TM + 1, nt_n = (p.n - 1) / TN + 1;
     // An XCD takes consecutive ids; they walk groups of 8 tiles of rows, so that the tiles in flight on it are about
     // as many rows as columns and share their panels in its L2.
     constexpr int GM = 8;
@@ -427,7 +427,7 @@ __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(OC
     constexpr int kElem = OUT == 0 ? 4 : 2, kRow = TN / WN * kElem, kPad = kRow + 16;  // bytes of a row, and in LDS
     constexpr int LR = kRow / 16, RL = 64 / LR;                                         // lanes per row, rows per store
     static_assert(32 * kPad * NWV <= (int)sizeof(smem), "a part of LDS for every wave");
-    const bool whole = p.c_ld * kElem % 16 == 0 && ((uintptr_t)p.c & 15) == 0 && n0 + wn + TN / WN <= p.n;
+    const bool whole = p.c_ld * kElem % 16 == 0 && ((uintptr_t)p.c & 15) == 0 && p.n - n0 - wn >= TN / WN;
     const bool aligned = p.c_ld % 4 == 0 && ((uintptr_t)p.c & (4 * kElem - 1)) == 0;
     asm volatile("s_barrier" ::: "memory");  // every wave has its last operands
     const uint32_t part = lds0 + wave * 32 * kPad;

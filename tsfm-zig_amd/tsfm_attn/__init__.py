@@ -1469,7 +1469,7 @@ class Kv8Pool:
         self.slots, self.pos = empty(max_tokens, t=torch.int64), empty(max_tokens)
         self.items = torch.full((_kv8_items(requests, max_tokens), 2), -1, dtype=torch.int32, device=device)
         self.status = torch.zeros(4, dtype=torch.int32, device=device)
-        self._workspace = None
+        self._workspace, self._home = None, 0
 
     @staticmethod
     def _check(rc: int) -> None:
@@ -1493,9 +1493,16 @@ class Kv8Pool:
 
             heads = q.numel() // max(1, q.shape[0]) // self.cache.head_dim
             n = kv8_attend_workspace(self.cache, heads, q.shape[0], max_new, max_len, stream)
-            if n > 0 and (self._workspace is None or self._workspace.numel() < n):
-                self._workspace = torch.empty(n, dtype=torch.uint8, device=q.device)
-            workspace = self._workspace
+            if n > 0:
+                _want(not torch.cuda.is_current_stream_capturing(), "a captured step needs a workspace of its own")
+                current = torch.cuda.current_stream(q.device)
+                if self._workspace is None or self._workspace.numel() < n:
+                    self._workspace, self._home = torch.empty(n, dtype=torch.uint8, device=q.device), current.cuda_stream
+                raw = _raw_stream(q, stream)
+                if raw != self._home:  # when a larger one takes its place, its memory waits for this stream too
+                    self._workspace.record_stream(torch.cuda.ExternalStream(raw, device=q.device) if raw else
+                                                  torch.cuda.default_stream(q.device))
+                workspace = self._workspace
         self._check(kv8_attend(self.cache, q, o, self.cu_tokens, scale=scale, max_new=max_new, max_len=max_len,
                                workspace=workspace, stream=stream))
 
