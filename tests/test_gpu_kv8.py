@@ -706,6 +706,28 @@ def test_many_rows_no_numbers(ta, gpu_ready, code, dtype, d):
         _check_attend(torch, pool, model, [news, news], q, o, d ** -0.5, dtype, kv, skip=(0,))
 
 
+@pytest.mark.parametrize("code,dtype,d,heads,kv", [("e4m3", "bf16", 64, 16, 16), ("i8", "f16", 64, 48, 4),
+                                                   ("e4m3", "f16", 128, 48, 4), ("i8", "bf16", 128, 12, 12)])
+@pytest.mark.parametrize("R", [13, 32])
+def test_requests_taken_by_length(ta, gpu_ready, code, dtype, d, heads, kv, R):
+    """Enough work that long requests go first: lengths that repeat, requests without tokens and new ones."""
+    torch = _t()
+    rng = np.random.default_rng(R + d + heads)
+    held = [int(n) for n in rng.choice([0, 0, 1, 64, 130, 130, 250, 333], R)]
+    news = [int(n) for n in rng.choice([0, 1, 7, 64, 70], R)] if R == 13 else [int(n) for n in rng.choice([0, 1, 9, 20], R)]
+    news[3] = 100
+    total = sum(news)
+    pool = _pool(ta, R, sum(-(-(a + b) // 64) for a, b in zip(held, news)), kv, d, code, dtype, 512, sum(held) + total + 1)
+    model = ref.Model(R, kv, d, code, pool.cache.blocks, 8)
+    for n_new in (held, news):
+        t = sum(n_new)
+        _step(torch, pool, model, n_new, _tokens(rng, t, kv, d, dtype), _tokens(rng, t, kv, d, dtype), dtype)
+    q = _round(rng.standard_normal((total, heads, d)), dtype)
+    o = torch.empty((total, heads, d), dtype=_dtype(dtype), device="cuda")
+    pool.attend(_dev(q, dtype), o, d ** -0.5, max_new=100, max_len=512)
+    _check_attend(torch, pool, model, news, q, o, d ** -0.5, dtype, kv)
+
+
 @pytest.mark.parametrize("d", [64, 128])
 def test_many_rows_of_short_requests(ta, gpu_ready, d):
     """Counts that do not fit, with many rows: clamped as for few, the rows before a request's start 0."""

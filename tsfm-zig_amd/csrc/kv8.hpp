@@ -61,6 +61,7 @@ struct Kv8Attend {
     int32_t rows;      // rows of a tile
     int32_t kernel;    // kAttend*
     int32_t once;      // the keys are read past the caches
+    int32_t longest_first;  // workgroups take the requests (64 at most) by length
     float* part;       // partial results: O (rows of o, heads, chunks, D), then (max, sum) pairs
 };
 constexpr int kAttendFew = 0, kAttendMany = 1;

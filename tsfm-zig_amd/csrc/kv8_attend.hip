@@ -87,6 +87,20 @@ __device__ __forceinline__ u32x4 ld_block(const uint8_t* p) {
 // (two spills) 144 where two take 134 (two requests of 262144).
 constexpr int few_waves(int d, int qt) { return d == 64 ? (qt == 1 ? 4 : 3) : 2; }
 
+// The i-th request in the order in which workgroups take them; the i-th longest where the host asks for it.
+__device__ __forceinline__ int nth_request(const Kv8Attend& p, int i) {
+    if (!p.longest_first) return i;
+    const int n = p.c.requests, lane = threadIdx.x & 63;
+    const int len = lane < n ? p.c.len[lane] : INT32_MIN;
+    int before = 0;
+    for (int j = 0; j < n; j++) {
+        const int other = __builtin_amdgcn_readlane(len, j);
+        before += other > len || (other == len && j < lane);
+    }
+    asm volatile("" : "+v"(before));  // opaque: merged with what follows, the ranking costs the loops there registers
+    return __builtin_ctzll(__ballot(lane < n && before == i));
+}
+
 template <int CODE, bool BF16, int D, int QT, bool ONCE>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(few_waves(D, QT), few_waves(D, QT)))) void attend_few(
     Kv8Attend p) {
@@ -115,7 +129,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(few_wav
     id /= c.heads;
     const int tile0 = id % p.tiles;
     id /= p.tiles;
-    const int r = id % c.requests, ck = id / c.requests;
+    const int r = nth_request(p, id % c.requests), ck = id / c.requests;
     const Span s = request_span(p.cu_tokens, c.len, r, p.max_tokens, c.width);
     const int G = p.group;
     const int64_t rows = (int64_t)s.n * G;
@@ -459,8 +473,9 @@ __global__ __launch_bounds__(64 * many_waves(D)) __attribute__((amdgpu_waves_per
     int id = idx / p.tiles * 8 + (blockIdx.x & 7);
     const int h = id % c.heads;
     id /= c.heads;
-    const int r = id % c.requests, ck = id / c.requests;
+    const int ck = id / c.requests;
     if (ck >= p.chunks) return;
+    const int r = nth_request(p, id % c.requests);
     const Span s = request_span(p.cu_tokens, c.len, r, p.max_tokens, c.width);
     const int G = p.group;
     const int64_t rows = (int64_t)s.n * G;
@@ -897,11 +912,17 @@ int64_t kv8_attend_plan(Kv8Attend& p, int head_dim, int max_new, int max_len, in
     // (two requests of 262144 tokens, 8 heads of 128: 384 workgroups 134 us, 768 147, 1536 163; 32 requests of up to
     // 2048 tokens, 16 heads of 64: unsplit 18.3 us, in two with the join 20.2). Chunks are 8 to 128 blocks: shorter ones
     // are all start and merge, and a longer one would keep a single workgroup busy after the others.
-    const int64_t chunks_wanted = std::max<int64_t>(1, (int64_t)cus * (p.kernel == kAttendMany ? head_dim == 64 ? 2 : 1 : few_waves(head_dim, p.rows / 16)) / base);
+    const int64_t resident = (int64_t)cus * (p.kernel == kAttendMany ? head_dim == 64 ? 2 : 1 : few_waves(head_dim, p.rows / 16));
+    const int64_t chunks_wanted = std::max<int64_t>(1, resident / base);
     const int64_t chunk = std::min<int64_t>(128, std::max<int64_t>(8, (blocks + chunks_wanted - 1) / chunks_wanted));
     const int64_t chunks = (blocks + chunk - 1) / chunk;
     p.chunk = (int32_t)chunk;
     p.chunks = (int32_t)chunks;
+    // Where workgroups fill the CUs, the long requests first leave short ones for the end (16 requests of up to 4096
+    // tokens, 128 dims: 128 rows 55 -> 46 us, 1024 171 -> 157, 2048 250 -> 200; four of up to 2048 new over 8192 486 ->
+    // 471; the other way four, 512 rows 41.8 -> 44.1). With room left the ranking only costs (32 requests of one token 20.8
+    // -> 21.4), and of more than 32 requests the last ones weigh little (64, 2048 rows: 727 -> 739).
+    p.longest_first = p.c.requests > 1 && p.c.requests <= 32 && base * chunks >= resident;
     if ((base + 8 * p.tiles) * chunks > INT32_MAX || (int64_t)p.max_tokens * p.heads > INT32_MAX) return -1;
     return chunks == 1 ? 0 : (int64_t)p.max_tokens * p.heads * chunks * (head_dim + 2) * 4;
 }
