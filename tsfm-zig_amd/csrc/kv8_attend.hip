@@ -421,7 +421,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(few_wav
 // them, so the weights go from the scores' registers straight into the second product.
 // A step computes the next block's scores beside this block's exponentials, and this block's second product beside the
 // decoding, one product and a few vector instructions at a time, its operands read from LDS a product ahead (products and
-// vector work one after the other, operands read where they were needed: 555 us where this takes 473, four requests of up
+// vector work one after the other, operands read where they were needed: 555 us where this took 473, four requests of up
 // to 2048 new tokens over 8192, 32 heads of 128 dims, 8 in the cache; 494 GFLOP). Bound by the issue of two waves a SIMD:
 // each unit is busy 40 to 45 % of the time; without the exponentials it takes 7 % less,
 // without the decoding 14 %, without half of the products 18 %.

@@ -1322,6 +1322,16 @@ def _rows_of(x: Any, what: str, width: int) -> int:
     return step[0]
 
 
+def _matrix(x: Any, what: str, rows: int, width: int) -> int:
+    """``_rows_of`` for a tensor that has `rows` rows."""
+    step = x.stride()
+    if x.shape == (rows, width) and step[1] == 1 and x.is_cuda:
+        return step[0]
+    if x.shape[:1] != (rows,):
+        raise ValueError(f"{what}: {rows} rows")
+    return _rows_of(x, what, width)
+
+
 def _kv8_items(requests: int, tokens: int) -> int:
     """The most cache blocks that `tokens` new tokens of `requests` requests touch (the rows of ``items``)."""
     return min(tokens, tokens // KV8_BLOCK + 2 * requests)
@@ -1516,13 +1526,13 @@ def f8_quantize(x, codes, scales, group_rows: int = 1, stream=None) -> int:
     ty = _types()
     rows, cols = x.shape
     groups = -(-cols // 128)
-    if not (codes.shape == x.shape and codes.dtype is ty.e4m3):
-        raise ValueError("codes: torch.float8_e4m3fn in x's shape")
-    if not (scales.dtype is ty.f32 and scales.shape[0] == (rows if group_rows == 1 else -(-rows // group_rows))):
-        raise ValueError("scales: f32, one row per group of rows")
+    if not (codes.dtype is ty.e4m3 and scales.dtype is ty.f32):
+        raise ValueError("codes: torch.float8_e4m3fn, scales: f32")
     args = _F8_QUANTIZE_PACK.pack(_dtype_code(x), rows, cols, group_rows, DEVICE_PTRS, x.data_ptr(),
-                                  _rows_of(x, "x", cols), codes.data_ptr(), _rows_of(codes, "codes", cols),
-                                  scales.data_ptr(), _rows_of(scales, "scales", groups), _raw_stream(x, stream))
+                                  _matrix(x, "x", rows, cols), codes.data_ptr(), _matrix(codes, "codes", rows, cols),
+                                  scales.data_ptr(),
+                                  _matrix(scales, "scales", rows if group_rows == 1 else -(-rows // group_rows), groups),
+                                  _raw_stream(x, stream))
     return load().tsfm_f8_quantize(args)
 
 
@@ -1534,12 +1544,11 @@ def f8_gemm_nt(a, a_scales, b, b_scales, c, stream=None) -> int:
     kb = -(-k // 128)
     if not (a.dtype is ty.e4m3 and b.dtype is ty.e4m3 and a_scales.dtype is ty.f32 and b_scales.dtype is ty.f32):
         raise ValueError("a and b: torch.float8_e4m3fn, their scales f32")
-    if not (a_scales.shape[0] == m and b_scales.shape[0] == -(-n // 128) and c.shape[0] == m):
-        raise ValueError("a_scales: (m, ceil(k / 128)); b_scales: (ceil(n / 128), ceil(k / 128)); c: (m, n)")
-    args = _F8_GEMM_PACK.pack(m, n, k, _dtype_code(c), DEVICE_PTRS, a.data_ptr(), _rows_of(a, "a", k),
-                              a_scales.data_ptr(), _rows_of(a_scales, "a_scales", kb), b.data_ptr(),
-                              _rows_of(b, "b", k), b_scales.data_ptr(), _rows_of(b_scales, "b_scales", kb),
-                              c.data_ptr(), _rows_of(c, "c", n), _raw_stream(a, stream))
+    args = _F8_GEMM_PACK.pack(m, n, k, _dtype_code(c), DEVICE_PTRS, a.data_ptr(), _matrix(a, "a", m, k),
+                              a_scales.data_ptr(), _matrix(a_scales, "a_scales", m, kb), b.data_ptr(),
+                              _matrix(b, "b", n, k), b_scales.data_ptr(),
+                              _matrix(b_scales, "b_scales", -(-n // 128), kb), c.data_ptr(), _matrix(c, "c", m, n),
+                              _raw_stream(a, stream))
     return load().tsfm_f8_gemm_nt(args)
 
 
