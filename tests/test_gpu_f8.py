@@ -250,6 +250,57 @@ def test_nothing_to_do(ta, gpu_ready):
     assert ta.f8_quantize(torch.empty((0, 128), device="cuda"), e, s) == ta.OK
 
 
+def test_captured_products(ta, gpu_ready):
+    """Quantisation and products of every kernel in one graph, replayed with other inputs and eager work between, and
+    the same calls on a second stream at the same time: each result as the eager one."""
+    torch = _t()
+    rng = np.random.default_rng(61)
+    shapes = [(1, 1000, 1024), (40, 500, 400), (300, 2000, 1040), (900, 1300, 640), (3500, 4200, 256)]
+    calls = []
+    for m, n, k in shapes:
+        _, _, _, _, _, b, _, sb = _operands(rng, 1, n, k)
+        calls.append((torch.empty((m, k), dtype=torch.bfloat16, device="cuda"), b, sb,
+                      torch.empty((m, k), dtype=torch.float8_e4m3fn, device="cuda"),
+                      torch.empty((m, -(-k // 128)), device="cuda"),
+                      torch.empty((m, n), dtype=torch.bfloat16 if n % 1000 else torch.float32, device="cuda")))
+
+    def run(outs, stream=None):
+        for (x, b, sb, a, sa, _), c in zip(calls, outs):
+            assert ta.f8_quantize(x, a, sa, stream=stream) == ta.OK
+            assert ta.f8_gemm_nt(a, sa, b, sb, c, stream=stream) == ta.OK
+
+    def fill():
+        for x, *_ in calls:
+            x.copy_(torch.randn(x.shape, device="cuda") * 3)
+
+    fill()
+    graph, outs = torch.cuda.CUDAGraph(), [c for *_, c in calls]
+    with torch.cuda.graph(graph):
+        run(outs)
+    for _ in range(4):
+        fill()
+        for c in outs:
+            c.fill_(-7)
+        graph.replay()
+        torch.randn(1000, device="cuda").sum()
+        torch.cuda.synchronize()
+        eager = [torch.empty_like(c) for c in outs]
+        run(eager)
+        for c, w in zip(outs, eager):
+            assert torch.equal(c, w)
+    # products of the same codes on two streams at once
+    torch.cuda.synchronize()
+    side, other = torch.cuda.Stream(), [torch.empty_like(c) for c in outs]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for (_, b, sb, a, sa, _), c, w in zip(calls, other, eager):
+            assert ta.f8_gemm_nt(a, sa, b, sb, c, stream=side) == ta.OK
+            assert ta.f8_gemm_nt(a, sa, b, sb, w) == ta.OK
+    torch.cuda.synchronize()
+    for c, o, w in zip(outs, other, eager):
+        assert torch.equal(c, o) and torch.equal(c, w)
+
+
 def test_serving_layer_in_8_bits(ta, gpu_ready):
     """The operators as a server runs them: two decode steps and a prompt through q/k/v in one 8-bit product, cache,
     attention and the output product, against the same in float64 from the GPU's own 8-bit activations (each product and

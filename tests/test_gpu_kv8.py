@@ -729,6 +729,52 @@ def test_requests_taken_by_length(ta, gpu_ready, code, dtype, d, heads, kv, R):
 
 
 @pytest.mark.parametrize("d", [64, 128])
+def test_captured_chunks(ta, gpu_ready, d):
+    """A prompt's chunks (plan, append, attention of many rows) and the release of a request in one graph, replayed
+    while the lengths advance: every replay as the eager pool's step."""
+    torch = _t()
+    rng = np.random.default_rng(67)
+    kv, heads, dtype, R, n = 2, 36, "bf16", 2, 70
+
+    def make():
+        p = _pool(ta, R, 24, kv, d, "e4m3", dtype, 640, R * n)
+        new = torch.tensor([n, n - 13], dtype=torch.int32, device="cuda")
+        drop = torch.tensor([0, 1], dtype=torch.uint8, device="cuda")
+        x = torch.zeros((R * n, (heads + 2 * kv) * d), dtype=torch.bfloat16, device="cuda")
+        o = torch.zeros((R * n, heads * d), dtype=torch.bfloat16, device="cuda")
+        ws = torch.empty(max(16, ta.kv8_attend_workspace(p.cache, heads, R * n, n, 640)), dtype=torch.uint8, device="cuda")
+
+        def step():
+            p.step(new)
+            p.append(x[:, heads * d:(heads + kv) * d], x[:, (heads + kv) * d:])
+            p.attend(x[:, :heads * d], o, d ** -0.5, max_new=n, max_len=640, workspace=ws)
+            p.release(drop)
+
+        return p, x, o, step
+
+    eager, e_in, e_out, e_step = make()
+    pool, g_in, g_out, step = make()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(5):
+        x = _dev(rng.standard_normal(e_in.shape), dtype)
+        e_in.copy_(x)
+        g_in.copy_(x)
+        g_out.fill_(-7)
+        e_step()
+        graph.replay()
+        torch.randn(1000, device="cuda").sum()
+        torch.cuda.synchronize()
+        total = 2 * n - 13
+        assert torch.equal(g_out[:total], e_out[:total]) and not torch.isnan(g_out[:total]).any()
+        assert (g_out[total:] == -7).all()
+        assert torch.equal(pool.length, eager.length) and pool.length[1].item() == 0
+        assert torch.equal(pool.table, eager.table) and torch.equal(pool.free_count, eager.free_count)
+    assert pool.length[0].item() == 5 * n
+
+
+@pytest.mark.parametrize("d", [64, 128])
 def test_many_rows_of_short_requests(ta, gpu_ready, d):
     """Counts that do not fit, with many rows: clamped as for few, the rows before a request's start 0."""
     torch = _t()
