@@ -200,7 +200,8 @@ __global__ __launch_bounds__(256) void plan_fill(Kv8Plan p) {
 // One workgroup: 1024 requests a round; their blocks are counted (a wave per dropped request), placed by a
 // prefix sum, and copied.
 __global__ __launch_bounds__(PT) void release(Kv8Release p) {
-    __shared__ int s_n[PT], s_off[PT], s_wave[PW];
+    __shared__ int s_n[PT];
+    __shared__ long long s_off[PT], s_wave[PW];  // 64 bits: tables that name a block many times pass 32
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int count = min(max(*p.free_count, 0), p.blocks);
     auto valid = [&](int r, int j) {  // the pool block at entry j, or -1
@@ -227,16 +228,16 @@ __global__ __launch_bounds__(PT) void release(Kv8Release p) {
                 if (lane == 0) s_n[i] = have;
             }
             __syncthreads();
-            int inc = s_n[tid];
-            const int own = inc;
+            long long inc = s_n[tid];
+            const long long own = inc;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
-                const int up = __shfl_up(inc, o);
+                const long long up = __shfl_up(inc, o);
                 if (lane >= o) inc += up;
             }
             if (lane == 63) s_wave[wave] = inc;
             __syncthreads();
-            int tot = 0;
+            long long tot = 0;
             for (int w = 0; w < PW; w++) {
                 if (w < wave) inc += s_wave[w];
                 tot += s_wave[w];
