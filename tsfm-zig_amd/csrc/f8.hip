@@ -97,7 +97,7 @@ __device__ __forceinline__ u32x2 codes8(const float (&v)[8], float mul) {
 // Rows: 16 lanes per group of 128 values (8 each), four groups per wave. Bound by bytes.
 template <int DTYPE>
 __global__ __launch_bounds__(256) void quantize_rows(F8Quantize p) {
-    const int groups = (p.cols + KB - 1) / KB;
+    const int groups = (p.cols - 1) / KB + 1;
     const int64_t id = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4, total = (int64_t)p.rows * groups;
     const int l = threadIdx.x & 15;
     const int64_t row = id / groups;
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(256) void quantize_rows(F8Quantize p) {
 template <int DTYPE>
 __global__ __launch_bounds__(256) void quantize_tiles(F8Quantize p) {
     __shared__ float s_max[4];
-    const int groups = (p.cols + KB - 1) / KB;
+    const int groups = (p.cols - 1) / KB + 1;
     const int grp = blockIdx.x % groups;
     const int64_t row0 = (int64_t)(blockIdx.x / groups) * KB;
     const int l = threadIdx.x & 15, col = grp * KB + 8 * l;
@@ -519,7 +519,7 @@ hipError_t gemm(const F8Gemm& p, int cus, hipStream_t s) {
 
 template <int DTYPE>
 hipError_t quantize(const F8Quantize& p, hipStream_t s) {
-    const int64_t groups = (p.cols + KB - 1) / KB;
+    const int64_t groups = (p.cols - 1) / KB + 1;
     if (p.group_rows == 1) {
         const int64_t grid = (p.rows * groups + 15) / 16;
         if (grid > 0x7fffffff) return hipErrorInvalidValue;
