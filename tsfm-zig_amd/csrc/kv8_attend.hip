@@ -693,8 +693,9 @@ __global__ __launch_bounds__(64 * many_waves(D)) __attribute__((amdgpu_waves_per
             }
             const float off = lv - (m_run == kNegInf ? 0.f : m_run);
             u32x4 pf[4];
-            // Exponentials in a row, G pairs of them after every second product, and what they need and feed after the others:
-            // each change between them and other vector instructions costs several cycles.
+            // Exponentials in a row, G pairs of them after every second product, and what they need and feed after the others
+            // (alternating with multiply-adds an exponential takes 16 cycles, in a row 9; one at a time this kernel took the
+            // same, 482 us).
             constexpr int G = 16 / KS;
             float sum[2] = {0.f, 0.f}, w[2][2 * G];
             auto add = [&](int g) {
